@@ -642,6 +642,95 @@ int rlgan_td_error(const float* q, const float* q_next, int ld, const float* rew
 int rlgan_lstm_gates(const float* gates, const float* c_in, int m, int units, float forget_bias, float* c_out, float* h_out,
                      void* stream);
 
+/* ---- training and acting of a recurrent policy -----------------------------------------------------------
+ * Three operators that the reference has no counterpart of; they stand beside its LSTM cell (rlgan_lstm_gates), its softmax
+ * cross-entropy (rlgan_softmax_ce) and its Adam / RMSProp (rlgan_apply).  Element types of tensors that may be narrower than
+ * 32 bits: */
+enum { RLGAN_F32 = 0, RLGAN_BF16 = 1, RLGAN_F16 = 2 };
+
+/* Gated linear recurrence over sequences [batch][length][width]:
+ *     f_t = sigmoid(z_t),  p_t = 0 where starts[b][t] != 0, else h_{t-1} (h_{-1} = state),  h_t = p_t + (1 - f_t) (x_t - p_t)
+ * A sequence [b] ends at step lengths[b] (clamped to 0 .. length): outputs at and behind it are 0, the state stays.
+ * rlgan_seq_t: strides in elements between batch rows and between steps; channels lie next to each other.  Rows may begin at
+ * any element.  Outputs overlap no input (state_out may be state, dstate_in may be dstate).  The state is 32 bits whatever the
+ * type; sums run in 32 bits. */
+typedef struct { void* p; int64_t batch, time; } rlgan_seq_t;
+typedef struct {
+  int32_t batch, length, width, type;      /* type: RLGAN_F32 / RLGAN_BF16 / RLGAN_F16 of z, x, h and their gradients */
+  rlgan_seq_t z, x;                        /* device, read only */
+  const float* state;                      /* device [batch][width], or NULL: zeros */
+  const uint8_t* starts;                   /* device, one byte a step at starts[b * starts_batch + t * starts_time], or NULL */
+  int64_t starts_batch, starts_time;
+  const int32_t* lengths;                  /* device [batch], or NULL */
+} rlgan_scan_t;
+/* bytes of device memory that a call of that shape wants as its workspace (may be 0, workspace then NULL).  A workspace belongs to
+ * one call at a time. */
+int rlgan_gated_scan_workspace(int batch, int length, int width, int type, int backward, int64_t* bytes);
+/* h [batch][length][width] and the state behind each sequence's last step */
+int rlgan_gated_scan_forward(const rlgan_scan_t* s, rlgan_seq_t h, float* state_out, void* workspace, void* stream);
+/* Gradient: h of the forward pass, dh the gradient of h, dstate of the final state (NULL: zeros) -> dz, dx, and dstate_in of the
+ * state handed in:  g_t = dh_t + f_{t+1} keep_{t+1} g_{t+1},  dx = (1 - f) g,  dz = g (p - x) f (1 - f). */
+int rlgan_gated_scan_backward(const rlgan_scan_t* s, rlgan_seq_t h, rlgan_seq_t dh, const float* dstate, rlgan_seq_t dz, rlgan_seq_t dx,
+                              float* dstate_in, void* workspace, void* stream);
+
+/* Clipped policy loss over rows of action logits [rows][vocab] and, when dlogits is non-NULL, its gradient:
+ *     log p = log softmax(logits / temperature),  H = entropy,  r = exp(log p[a] - old_logp),  d = ref_logp - log p[a]
+ *     l = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^d - d - 1) - entropy_coef H,  loss = sum weights l
+ * logp, entropy, kl: the row's log p[a], H and e^d - d - 1 (0 without ref_logp).  A row is left out (zeros in every output, no
+ * share in the loss, whatever its other numbers) when its action is negative, its weight 0, its action not legal or the action's
+ * logit -inf.  Logits that are not legal are never used, whatever they hold.  An action >= vocab makes the row and the loss NaN.
+ * dlogits may be logits. */
+typedef struct {
+  int64_t rows;
+  int32_t vocab, type;
+  const void* logits; int64_t ld;          /* device, row stride in elements */
+  const void* actions; int32_t action_bytes;   /* device [rows], int32 (4) or int64 (8) */
+  const float *old_logp, *advantages;      /* device [rows] */
+  const float* weights;                    /* device [rows], or NULL: 1 / rows each */
+  const float* ref_logp;                   /* device [rows], or NULL: no KL term */
+  const uint8_t* legal; int64_t ld_legal;  /* device [rows][vocab] bytes, 0: not legal; or NULL */
+  double clip_low, clip_high, kl_coef, entropy_coef, temperature;
+  float *loss, *logp, *entropy, *kl;       /* device: [1], [rows] each */
+  void* dlogits; int64_t ld_d;             /* device, or NULL */
+} rlgan_policy_t;
+int rlgan_policy_loss_workspace(int64_t rows, int vocab, int type, int64_t* bytes);
+int rlgan_policy_loss(const rlgan_policy_t* p, void* workspace, void* stream);
+
+/* AdamW (decoupled weight decay) over a list of tensors:
+ *     g = grad * grad_scale,  m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *     p = p (1 - lr decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+ * Every tensor's state begins at a multiple of 64 in the flat state arrays (rlgan_adamw_tensor_t.offset).  state_bits 32: first
+ * and second hold m and v as floats.  state_bits 8: they hold one byte an element, first_exp and second_exp one byte for every 64
+ * elements: m as a sign and 7 bits, the root of v as 8 bits, floats of 3 and 4 mantissa bits that share the exponent of the largest
+ * of the 64 and count down from the top of its octave (rlgan_adamw_decode gives the values).  A block with a number that is not
+ * finite reads as NaN.
+ * chunks: device, (tensor, chunk of RLGAN_ADAMW_CHUNK elements within it) for every chunk of every tensor in order; chunk_begin:
+ * HOST, n_tensors + 1 places of the tensors' first chunks.  step: device counter of the steps done, advanced by the call; lr:
+ * device scalar; scalars: device scratch of 16 bytes. */
+#define RLGAN_ADAMW_CHUNK 2048
+typedef struct { void* param; int64_t count, offset; int32_t type, reserved; } rlgan_adamw_tensor_t;
+typedef struct {
+  int32_t n_tensors, state_bits;
+  const rlgan_adamw_tensor_t* tensors;     /* device [n_tensors] */
+  const int32_t* chunks;
+  const int64_t* chunk_begin;
+  void *first, *second;
+  uint8_t *first_exp, *second_exp;
+  const float* lr;
+  int32_t* step;
+  float* scalars;
+  double beta1, beta2, eps, weight_decay;
+} rlgan_adamw_t;
+/* grads, grad_types: HOST arrays of n_tensors device pointers and element types (any of the three, whatever the parameter's).
+ * grad_scale: device scalar or NULL.  skip: device byte or NULL; where it is not 0 the call changes nothing. */
+int rlgan_adamw_step(const rlgan_adamw_t* a, const void* const* grads, const uint8_t* grad_types, const float* grad_scale, const uint8_t* skip,
+                     void* stream);
+/* n (a multiple of 64) elements of the 8-bit state as floats m and v, and the state nearest to given ones */
+int rlgan_adamw_decode(const uint8_t* first, const uint8_t* second, const uint8_t* first_exp, const uint8_t* second_exp, int64_t n, float* m,
+                       float* v, void* stream);
+int rlgan_adamw_encode(const float* m, const float* v, int64_t n, uint8_t* first, uint8_t* second, uint8_t* first_exp, uint8_t* second_exp,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,9 +21,13 @@ from .pixel_gan import PixelDiscriminator, PixelGanTrainer, PixelGenerator, sing
 from .inverse_model import BatchNorm, StateActionPredictor
 from .pixel_ddpg import LSTMUnit, PixelActor, PixelCritic
 from .train_pixel import PixelAgent, PixelSettings, train_pixel, transfer_sparse_action
+from .recurrence import GatedUnit, gated_scan, gated_scan_backward, gated_step
+from .policy import PolicyLoss, policy_loss
+from .adamw import AdamW
 from .train import Agent, Settings, train, train_DDPG
 
 __all__ = ["Session", "placeholder", "set_random_seed", "Actor", "Critic", "Generator", "Discriminator", "Memory",
            "DDPGMemory", "ArmEnv", "VecArmEnv", "DeviceMemory", "FrameMemory", "PixelMemory", "PixelAgent", "PixelSettings", "train_pixel", "transfer_sparse_action", "FrameRef", "Decoder", "DeconvLayer", "DECODER", "PixelGenerator", "PixelDiscriminator", "PixelGanTrainer", "single_frame_encoder", "StateActionPredictor", "PixelActor", "LSTMUnit", "PixelCritic", "BatchNorm", "MT19937Device", "StepEngine", "GradExchange",
            "CuriousLearner", "LearnerConfig", "DeviceNet", "mlp_forward", "ConvEncoder", "ConvLayer", "DenseLayer", "DOOM_HEAD",
-           "universe_head", "Agent", "Settings", "train", "train_DDPG"]
+           "universe_head", "GatedUnit", "gated_scan", "gated_scan_backward", "gated_step", "PolicyLoss", "policy_loss", "AdamW", "Agent", "Settings",
+           "train", "train_DDPG"]

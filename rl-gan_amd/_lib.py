@@ -140,6 +140,36 @@ class ApplyJob(C.Structure):
                 ("reduce", C.POINTER(ReduceJob))]
 
 
+class SeqRef(C.Structure):
+    _fields_ = [("p", _fp), ("batch", C.c_int64), ("time", C.c_int64)]
+
+
+class Scan(C.Structure):
+    _fields_ = [("batch", _i32), ("length", _i32), ("width", _i32), ("type", _i32), ("z", SeqRef), ("x", SeqRef), ("state", _fp),
+                ("starts", _fp), ("starts_batch", C.c_int64), ("starts_time", C.c_int64), ("lengths", _fp)]
+
+
+class Policy(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("vocab", _i32), ("type", _i32), ("logits", _fp), ("ld", C.c_int64), ("actions", _fp),
+                ("action_bytes", _i32), ("old_logp", _fp), ("advantages", _fp), ("weights", _fp), ("ref_logp", _fp), ("legal", _fp),
+                ("ld_legal", C.c_int64), ("clip_low", C.c_double), ("clip_high", C.c_double), ("kl_coef", C.c_double),
+                ("entropy_coef", C.c_double), ("temperature", C.c_double), ("loss", _fp), ("logp", _fp), ("entropy", _fp), ("kl", _fp),
+                ("dlogits", _fp), ("ld_d", C.c_int64)]
+
+
+ADAMW_CHUNK, ADAMW_BLOCK = 2048, 64                              # RLGAN_ADAMW_CHUNK; elements that share an exponent
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [("param", _fp), ("count", C.c_int64), ("offset", C.c_int64), ("type", _i32), ("reserved", _i32)]
+
+
+class AdamWState(C.Structure):
+    _fields_ = [("n_tensors", _i32), ("state_bits", _i32), ("tensors", _fp), ("chunks", _fp), ("chunk_begin", _fp), ("first", _fp),
+                ("second", _fp), ("first_exp", _fp), ("second_exp", _fp), ("lr", _fp), ("step", _fp), ("scalars", _fp),
+                ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -236,6 +266,14 @@ PROTOTYPES = {
     "rlgan_dense_backward_input_split": [_vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp],
     "rlgan_dense_backward_weights": [_vp, _i, _vp, _i, _vp, _i, _i, _i, _vp, _i, _vp],
     "rlgan_dense_backward_kernel": [_vp, _i, _vp, _i, _vp, _i, _i, _i, _vp, _i, _vp],
+    "rlgan_gated_scan_workspace": [_i, _i, _i, _i, _i, C.POINTER(C.c_int64)],
+    "rlgan_gated_scan_forward": [C.POINTER(Scan), SeqRef, _vp, _vp, _vp],
+    "rlgan_gated_scan_backward": [C.POINTER(Scan), SeqRef, SeqRef, _vp, SeqRef, SeqRef, _vp, _vp, _vp],
+    "rlgan_policy_loss_workspace": [C.c_int64, _i, _i, C.POINTER(C.c_int64)],
+    "rlgan_policy_loss": [C.POINTER(Policy), _vp, _vp],
+    "rlgan_adamw_step": [C.POINTER(AdamWState), _vp, _vp, _vp, _vp, _vp],
+    "rlgan_adamw_decode": [_vp, _vp, _vp, _vp, C.c_int64, _vp, _vp, _vp],
+    "rlgan_adamw_encode": [_vp, _vp, C.c_int64, _vp, _vp, _vp, _vp, _vp],
 }
 
 for _name, _args in PROTOTYPES.items():

@@ -1,0 +1,154 @@
+"""AdamW over any list of tensors in one pass, with the moments in 32 or in 8 bits: the optimizer of layers that are plain
+tensors (`DenseLayer.canon`, `GatedUnit.gates.canon`, a caller's own), beside the Adam and RMSProp of the packed networks
+(`rlgan_apply`, DDPG.py:69,145, Curious_GAN.py:37-42)."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import List, Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from ._lib import ADAMW_BLOCK, ADAMW_CHUNK, AdamWState, AdamWTensor, check, lib
+from .tensors import TYPES, byte_range, first_device, guard, need, on_device, stream_of, type_code
+
+
+class AdamW:
+    """p = p (1 - lr decay) - lr m^ / (sqrt(v^) + eps) with m^, v^ the moments corrected for their zero start, decay apart from them.
+
+    params: contiguous float32, bfloat16 or float16 tensors of one GPU, in any mixture, that share no memory.  The update is
+    computed in float32 and rounded to the parameter's type (to nearest: 16-bit weights lose updates below half a step).
+    state_bits 32: moments as float32, 8 bytes a parameter.  state_bits 8: one byte each for m and the root of v, 2.03 bytes a
+    parameter; every 64 elements share an exponent under which codes reach 16 octaves, rounded by at most 2^-4 (m) and 2^-5 (root).
+    `lr` and `steps` are device scalars that the kernels read, so that a captured step follows `set_lr` and counts on."""
+
+    def __init__(self, params: Sequence[torch.Tensor], lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, state_bits: int = 32):
+        self.params: List[torch.Tensor] = list(params)
+        need(len(self.params) > 0, "no parameters")
+        need(state_bits in (8, 32), "state_bits: 8 or 32")
+        need(0 <= betas[0] < 1 and 0 <= betas[1] < 1, "betas: at least 0 and below 1")
+        need(lr >= 0 and eps >= 0 and weight_decay >= 0, "lr, eps and weight_decay: not negative")
+        self.device = dev = first_device(self.params[0], "params[0]")
+        self.betas, self.eps, self.weight_decay, self.state_bits = (float(betas[0]), float(betas[1])), float(eps), float(weight_decay), state_bits
+        for i, p in enumerate(self.params):
+            on_device(p, dev, f"params[{i}]")
+            type_code(p, f"params[{i}]")
+            need(p.is_contiguous(), f"params[{i}] is not contiguous")
+        spans = sorted(byte_range(p) + (i,) for i, p in enumerate(self.params) if p.numel())
+        for (_, hi, i), (lo, _, j) in zip(spans, spans[1:]):
+            need(hi <= lo, f"params[{i}] and params[{j}] share memory")
+        counts = np.array([p.numel() for p in self.params], np.int64)
+        padded = (counts + ADAMW_BLOCK - 1) // ADAMW_BLOCK * ADAMW_BLOCK
+        self.offsets = np.concatenate([[0], np.cumsum(padded)]).astype(np.int64)
+        self.size = int(self.offsets[-1])                        # elements of the flat state
+        n_chunks = (counts + ADAMW_CHUNK - 1) // ADAMW_CHUNK
+        need(int(n_chunks.sum()) < 1 << 31, "too many parameters")
+        self._chunk_begin = np.ascontiguousarray(np.concatenate([[0], np.cumsum(n_chunks)]).astype(np.int64))
+        which = np.repeat(np.arange(len(counts)), n_chunks)
+        table = np.stack([which, np.arange(len(which)) - self._chunk_begin[which]], 1).astype(np.int32)
+        self._ptrs = [p.data_ptr() for p in self.params]
+        records = (AdamWTensor * len(counts))(*[AdamWTensor(q, int(n), int(o), TYPES[p.dtype], 0)
+                                                for q, n, o, p in zip(self._ptrs, counts, self.offsets, self.params)])
+        up = lambda a: torch.from_numpy(a).to(dev)
+        self._records = up(np.frombuffer(bytes(records), np.uint8).copy())
+        self._chunks = up(table if len(table) else np.zeros((1, 2), np.int32))
+        n = max(self.size, ADAMW_BLOCK)
+        kind = torch.float32 if state_bits == 32 else torch.uint8
+        self.first, self.second = torch.zeros(n, dtype=kind, device=dev), torch.zeros(n, dtype=kind, device=dev)
+        self.first_exp = self.second_exp = None
+        if state_bits == 8:
+            self.first_exp = torch.zeros(n // ADAMW_BLOCK, dtype=torch.uint8, device=dev)
+            self.second_exp = torch.zeros_like(self.first_exp)
+        self.lr = torch.full((1,), float(lr), dtype=torch.float32, device=dev)
+        self.steps = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._scalars = torch.zeros(4, dtype=torch.float32, device=dev)
+        ptr = lambda t: None if t is None else t.data_ptr()
+        self._state = AdamWState(len(counts), state_bits, ptr(self._records), ptr(self._chunks), self._chunk_begin.ctypes.data, ptr(self.first),
+                                 ptr(self.second), ptr(self.first_exp), ptr(self.second_exp), ptr(self.lr), ptr(self.steps), ptr(self._scalars),
+                                 self.betas[0], self.betas[1], self.eps, self.weight_decay)
+
+    def set_lr(self, lr: float) -> None:
+        """The rate of the following steps, those of captured graphs among them."""
+        need(lr >= 0, "lr: not negative")
+        self.lr.fill_(float(lr))
+
+    def step(self, grads: Sequence[torch.Tensor], grad_scale: Optional[torch.Tensor] = None, skip: Optional[torch.Tensor] = None) -> None:
+        """One step.  grads: a gradient for every parameter, of its shape, in any of the three types.  grad_scale: float32
+        device scalar that multiplies the gradients (1 / loss scale, what clipping by a norm left).  skip: bool device scalar;
+        where it is True nothing changes (gradients of a scaled loss that overflowed)."""
+        need(len(grads) == len(self.params), f"{len(grads)} gradients for {len(self.params)} parameters")
+        n, dev = len(grads), self.device
+        pointers, types = (C.c_void_p * n)(), (C.c_uint8 * n)()
+        for i, (p, q, g) in enumerate(zip(self.params, self._ptrs, grads)):
+            code = TYPES.get(g.dtype)
+            if code is None or g.device != dev or g.shape != p.shape or not g.is_contiguous():
+                raise ValueError(f"grads[{i}]: a contiguous float32, bfloat16 or float16 tensor of shape {tuple(p.shape)} on {dev} is wanted")
+            if p.data_ptr() != q:
+                raise ValueError(f"params[{i}] has moved in memory since the optimizer was made")
+            pointers[i], types[i] = g.data_ptr(), code
+        p_scale = p_skip = None
+        if grad_scale is not None:
+            on_device(grad_scale, dev, "grad_scale")
+            need(grad_scale.dtype == torch.float32 and grad_scale.numel() == 1, "grad_scale: one float32 on the device")
+            p_scale = grad_scale.data_ptr()
+        if skip is not None:
+            on_device(skip, dev, "skip")
+            need(skip.dtype in (torch.bool, torch.uint8) and skip.numel() == 1, "skip: one bool on the device")
+            p_skip = skip.data_ptr()
+        with guard(dev):
+            check(lib.rlgan_adamw_step(C.byref(self._state), pointers, types, p_scale, p_skip, stream_of(dev)), "rlgan_adamw_step")
+
+    # ---- state -------------------------------------------------------------------------------------
+    def moments(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(m, v) as flat float32 tensors, every parameter's part beginning at a multiple of 64 (`views` cuts them out): the
+        state itself with 32 bits, the values that the codes stand for with 8."""
+        if self.state_bits == 32:
+            return self.first[:self.size], self.second[:self.size]
+        m, v = torch.empty(self.size, dtype=torch.float32, device=self.device), torch.empty(self.size, dtype=torch.float32, device=self.device)
+        if self.size:
+            with guard(self.device):
+                check(lib.rlgan_adamw_decode(self.first.data_ptr(), self.second.data_ptr(), self.first_exp.data_ptr(), self.second_exp.data_ptr(),
+                                             self.size, m.data_ptr(), v.data_ptr(), stream_of(self.device)), "rlgan_adamw_decode")
+        return m, v
+
+    def views(self, flat: torch.Tensor) -> List[torch.Tensor]:
+        """The parts of a flat state tensor in the parameters' shapes."""
+        return [flat[int(o):int(o) + p.numel()].view(p.shape) for o, p in zip(self.offsets, self.params)]
+
+    def load_moments(self, first: torch.Tensor, second: torch.Tensor, steps: int) -> None:
+        """Sets the state from flat float32 m and v as `moments` lays them out (what lies between the parameters is not used) and
+        the number of steps done; with 8 bits, to the nearest codes."""
+        for name, t in (("first", first), ("second", second)):
+            on_device(t, self.device, name)
+            need(t.dtype == torch.float32 and t.shape == (self.size,), f"{name}: float32 of shape [{self.size}]")
+        need(0 <= int(steps) < 1 << 31, "steps: not negative")
+        clean = [torch.zeros(max(self.size, ADAMW_BLOCK), dtype=torch.float32, device=self.device) for _ in range(2)]
+        for to, t in zip(clean, (first, second)):
+            for a, b in zip(self.views(to), self.views(t)):
+                a.copy_(b)
+        if self.state_bits == 32:
+            self.first.copy_(clean[0])
+            self.second.copy_(clean[1])
+        else:
+            with guard(self.device):
+                check(lib.rlgan_adamw_encode(clean[0].data_ptr(), clean[1].data_ptr(), clean[0].numel(), self.first.data_ptr(),
+                                             self.second.data_ptr(), self.first_exp.data_ptr(), self.second_exp.data_ptr(),
+                                             stream_of(self.device)), "rlgan_adamw_encode")
+        self.steps.fill_(int(steps))
+
+    def state_dict(self) -> dict:
+        """A copy of everything a step changes beside the parameters, as it is held."""
+        d = {"first": self.first.clone(), "second": self.second.clone(), "steps": self.steps.clone(), "lr": self.lr.clone()}
+        if self.state_bits == 8:
+            d["first_exp"], d["second_exp"] = self.first_exp.clone(), self.second_exp.clone()
+        return d
+
+    def load_state_dict(self, d: dict) -> None:
+        own = ["first", "second", "steps", "lr"] + (["first_exp", "second_exp"] if self.state_bits == 8 else [])
+        need(sorted(d) == sorted(own), f"state: {sorted(own)} are wanted, got {sorted(d)}")
+        for k in own:
+            t = getattr(self, k)
+            need(d[k].dtype == t.dtype and d[k].shape == t.shape, f"state[{k!r}]: {t.dtype} of shape {tuple(t.shape)} is wanted")
+        for k in own:
+            getattr(self, k).copy_(d[k])

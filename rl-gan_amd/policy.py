@@ -1,0 +1,95 @@
+"""Clipped policy loss over action logits, with a KL term to a reference policy and an entropy bonus, and its gradient, in one
+pass over the logits.  For policies over discrete actions (or tokens), beside the deterministic actors' gradients
+(DDPG.py:97, Conv_model.py:569-784) and the inverse model's softmax cross-entropy (Conv_model.py:801,818)."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+
+from ._lib import Policy, check, lib
+from .tensors import apart, first_device, guard, need, on_device, own_elements, stream_of, type_code, vector, workspace
+
+
+class PolicyLoss(NamedTuple):
+    loss: torch.Tensor                        # [] float32
+    logp: torch.Tensor                        # [rows] float32: log-probability of each row's action
+    entropy: torch.Tensor                     # [rows]
+    kl: torch.Tensor                          # [rows]: e^d - d - 1 with d = ref_logp - logp; 0 without ref_logp
+    dlogits: Optional[torch.Tensor]           # gradient of the loss, in the logits' type
+
+
+def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor, *,
+                weights: Optional[torch.Tensor] = None, ref_logp: Optional[torch.Tensor] = None, legal: Optional[torch.Tensor] = None,
+                clip: Union[float, Tuple[float, float]] = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0, temperature: float = 1.0,
+                grad: bool = True, out: Optional[torch.Tensor] = None) -> PolicyLoss:
+    """loss = sum_i w_i [ -min(r_i A_i, clip(r_i, 1 - low, 1 + high) A_i) + kl_coef k_i - entropy_coef H_i ]
+
+    with r = exp(log p[a] - old_logp), p = softmax(logits / temperature) over the legal actions, k the estimate
+    e^d - d - 1, d = ref_logp - log p[a], of the divergence from a reference policy, and H the entropy of p.
+
+    logits [rows, actions]: float32, bfloat16 or float16, any row stride.  actions: int32 or int64 [rows].  old_logp, advantages,
+    weights, ref_logp: float32 [rows]; weights default to 1 / rows each (a mean over counted rows: weights = mask / mask.sum()).
+    legal: bool or uint8 [rows, actions], False for actions that cannot be chosen.  clip: one bound or (low, high).
+    out: tensor for the gradient, or the logits themselves to overwrite them.
+
+    A row is left out, with zeros in every output, where its action is negative (padding), its weight is 0, or its action is not
+    legal or has a logit of -inf.  An action at or above the number of actions makes the loss and its row NaN."""
+    dev = first_device(logits, "logits")
+    code = type_code(logits, "logits")
+    need(logits.dim() == 2 and (logits.shape[1] <= 1 or logits.stride(1) == 1), "logits: [rows, actions] with a row's logits next to each other")
+    rows, vocab = logits.shape
+    need(vocab > 0 and vocab < 1 << 31 and rows < 1 << 31, "logits: at least one action, fewer than 2^31 actions and rows")
+    on_device(actions, dev, "actions")
+    need(actions.dtype in (torch.int32, torch.int64) and actions.shape == (rows,) and actions.is_contiguous(),
+         "actions: contiguous int32 or int64 of shape [rows]")
+    low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
+    need(0 <= low <= 1 and high >= 0, "clip: bounds of at least 0, the lower one at most 1")
+    need(temperature > 0 and temperature < float("inf"), "temperature has to be positive")
+    p_old, p_adv = vector(old_logp, (rows,), dev, "old_logp"), vector(advantages, (rows,), dev, "advantages")
+    need(p_old is not None and p_adv is not None, "old_logp and advantages are wanted")
+    p_w, p_ref = vector(weights, (rows,), dev, "weights"), vector(ref_logp, (rows,), dev, "ref_logp")
+    p_legal, ld_legal = None, 0
+    if legal is not None:
+        on_device(legal, dev, "legal")
+        need(legal.dtype in (torch.bool, torch.uint8) and legal.shape == logits.shape and (vocab == 1 or legal.stride(1) == 1),
+             "legal: bool or uint8 of the logits' shape, a row's flags next to each other")
+        p_legal, ld_legal = legal.data_ptr(), _row_stride(legal, vocab)
+        need(ld_legal >= vocab or rows == 1 or legal.stride(0) == 0, "legal: rows that overlap")
+    ld = _row_stride(logits, vocab)
+    need(ld >= vocab, "logits: rows that overlap")
+    d = None
+    if grad:
+        d = out
+        if d is None:
+            d = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+        else:
+            on_device(d, dev, "out")
+            need(d.dtype == logits.dtype and d.shape == logits.shape and (vocab == 1 or d.stride(1) == 1),
+                 "out: the logits' type and shape, a row's values next to each other")
+            if d.data_ptr() == logits.data_ptr() and d.stride() == logits.stride():
+                own_elements(d, "out")
+                apart(d, (actions, old_logp, advantages, weights, ref_logp, legal), "out")
+            else:
+                apart(d, (logits, actions, old_logp, advantages, weights, ref_logp, legal), "out")
+    else:
+        need(out is None, "out: there is no gradient to write with grad=False")
+    if rows == 0:
+        none = torch.zeros(0, dtype=torch.float32, device=dev)
+        return PolicyLoss(torch.zeros((), dtype=torch.float32, device=dev), none, none.clone(), none.clone(), d)
+    with guard(dev):
+        stats = torch.empty((4, rows), dtype=torch.float32, device=dev)
+        size = C.c_int64()
+        check(lib.rlgan_policy_loss_workspace(rows, vocab, code, C.byref(size)), "rlgan_policy_loss_workspace")
+        ws = workspace(size.value, dev)
+        base = stats.data_ptr()
+        args = Policy(rows, vocab, code, logits.data_ptr(), ld, actions.data_ptr(), actions.element_size(), p_old, p_adv, p_w, p_ref, p_legal,
+                      ld_legal, low, high, kl_coef, entropy_coef, temperature, base, base + 4 * rows, base + 8 * rows, base + 12 * rows,
+                      None if d is None else d.data_ptr(), 0 if d is None else _row_stride(d, vocab))
+        check(lib.rlgan_policy_loss(C.byref(args), ws.data_ptr(), stream_of(dev)), "rlgan_policy_loss")
+    return PolicyLoss(stats[0, 0], stats[1], stats[2], stats[3], d)
+
+
+def _row_stride(t: torch.Tensor, vocab: int) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), vocab)

@@ -1,0 +1,182 @@
+"""Gated linear recurrence over time: the trainable memory of a recurrent policy, beside the reference's `lstm_unit`
+(Conv_model.py:67-99), which gets no gradient.
+
+    f_t = sigmoid(z_t),   p_t = 0 where an episode starts at t, else h_{t-1},   h_t = p_t + (1 - f_t) (x_t - p_t)
+
+z and x depend on the inputs alone, so a whole sequence is one scan (`gated_scan`, `gated_scan_backward`) and acting is one step
+(`gated_step`).  Sequences are [batch, time, width] tensors of float32, bfloat16 or float16 with channels next to each other
+and any other strides (time-major data goes in as a transposed view, the two halves of one dense product as slices); the state
+[batch, width] is float32 whatever their type."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import numpy as np
+import torch
+
+from ._lib import Scan, SeqRef, check, lib
+from .conv import DenseLayer
+from .tensors import apart, first_device, guard, need, on_device, stream_of, type_code, vector, workspace
+
+
+def _seq(t: torch.Tensor, shape, dtype, dev, name: str) -> SeqRef:
+    on_device(t, dev, name)
+    if t.dtype != dtype or t.shape != shape:
+        raise ValueError(f"{name}: {dtype} of shape {tuple(shape)} is wanted, got {t.dtype} {tuple(t.shape)}")
+    if t.stride(2) != 1 and shape[2] > 1:
+        raise ValueError(f"{name}: channels have to lie next to each other (strides {t.stride()})")
+    return SeqRef(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _scan(z, x, state, starts, lengths) -> Tuple[Scan, torch.device]:
+    dev = first_device(z, "z")
+    code = type_code(z, "z")
+    need(z.dim() == 3, "z and x are [batch, time, width]")
+    shape = z.shape
+    b, n, d = shape
+    need(b * d <= 1 << 31 and n < 1 << 31, "at most 2^31 units and steps")
+    st = None
+    sb = ss = 0
+    if starts is not None:
+        on_device(starts, dev, "starts")
+        need(starts.dtype in (torch.bool, torch.uint8) and starts.shape == shape[:2], "starts: bool or uint8 of shape [batch, time]")
+        st, sb, ss = starts.data_ptr(), starts.stride(0), starts.stride(1)
+    return Scan(b, n, d, code, _seq(z, shape, z.dtype, dev, "z"), _seq(x, shape, z.dtype, dev, "x"), vector(state, (b, d), dev, "state"), st,
+                sb, ss, vector(lengths, (b,), dev, "lengths", torch.int32)), dev
+
+
+def _output(out, like, others, name):
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    apart(out, others, name)
+    return out
+
+
+def _workspace(s: Scan, backward: int, dev) -> Optional[torch.Tensor]:
+    size = C.c_int64()
+    check(lib.rlgan_gated_scan_workspace(s.batch, s.length, s.width, s.type, backward, C.byref(size)), "rlgan_gated_scan_workspace")
+    return workspace(size.value, dev)
+
+
+def gated_scan(z: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tensor] = None, *, starts: Optional[torch.Tensor] = None,
+               lengths: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(h, state): h [batch, time, width] in z's type (in `out` if given) and the state behind each sequence's last step.
+
+    state: what the sequences continue from (zeros if None).  starts: bool [batch, time], True where an episode begins: nothing
+    from before reaches that step.  lengths: int32 [batch], steps of each sequence (clamped to 0 .. time); h is 0 at and behind
+    a sequence's end, whatever z and x hold there, and the state is the one at its end."""
+    s, dev = _scan(z, x, state, starts, lengths)
+    h = _output(out, z, (z, x, state, starts, lengths), "out")
+    ref = _seq(h, z.shape, z.dtype, dev, "out")
+    if z.numel() == 0:
+        return h, torch.zeros((s.batch, s.width), dtype=torch.float32, device=dev) if state is None else state.clone()
+    with guard(dev):
+        last = torch.empty((s.batch, s.width), dtype=torch.float32, device=dev)
+        ws = _workspace(s, 0, dev)
+        check(lib.rlgan_gated_scan_forward(C.byref(s), ref, last.data_ptr(), None if ws is None else ws.data_ptr(), stream_of(dev)),
+              "rlgan_gated_scan_forward")
+    return h, last
+
+
+def gated_scan_backward(dh: torch.Tensor, z: torch.Tensor, x: torch.Tensor, h: torch.Tensor, state: Optional[torch.Tensor] = None, *,
+                        starts: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                        dstate: Optional[torch.Tensor] = None,
+                        out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dz, dx, dstate_in) of `gated_scan` for the gradient dh of h and dstate of the returned state (zeros if None).
+
+    h: what the forward pass returned, in its type (for 16 bits it carries that type's rounding into dz: the alternative is a
+    second forward scan).  out: tensors for dz and dx, which may be the halves of one buffer.  At and behind a sequence's end dz
+    and dx are 0, whatever dh holds there."""
+    s, dev = _scan(z, x, state, starts, lengths)
+    rh, rdh = _seq(h, z.shape, z.dtype, dev, "h"), _seq(dh, z.shape, z.dtype, dev, "dh")
+    dst = vector(dstate, (s.batch, s.width), dev, "dstate")
+    inputs = (z, x, h, dh, state, starts, lengths, dstate)
+    if out is not None:
+        need(len(out) == 2, "out: (dz, dx)")
+        _halves_apart(*out)
+    dz = _output(None if out is None else out[0], z, inputs, "out[0]")
+    dx = _output(None if out is None else out[1], z, inputs, "out[1]")
+    rdz, rdx = _seq(dz, z.shape, z.dtype, dev, "out[0]"), _seq(dx, z.shape, z.dtype, dev, "out[1]")
+    if z.numel() == 0:
+        return dz, dx, torch.zeros((s.batch, s.width), dtype=torch.float32, device=dev) if dstate is None else dstate.clone()
+    with guard(dev):
+        first = torch.empty((s.batch, s.width), dtype=torch.float32, device=dev)
+        ws = _workspace(s, 1, dev)
+        check(lib.rlgan_gated_scan_backward(C.byref(s), rh, rdh, dst, rdz, rdx, first.data_ptr(), None if ws is None else ws.data_ptr(),
+                                            stream_of(dev)), "rlgan_gated_scan_backward")
+    return dz, dx, first
+
+
+def _halves_apart(a: torch.Tensor, b: torch.Tensor) -> None:
+    """Two outputs either lie in memory of their own or are slices side by side in the rows of one buffer."""
+    need(isinstance(a, torch.Tensor) and isinstance(b, torch.Tensor) and a.dim() == 3 and a.shape == b.shape, "out: two tensors of z's shape")
+    if a.stride() == b.stride() and a.numel():
+        gap, row = abs(a.data_ptr() - b.data_ptr()), a.shape[2] * a.element_size()
+        rows = [s * a.element_size() for s, n in zip(a.stride()[:2], a.shape[:2]) if n > 1]
+        if gap >= row and all(gap + row <= r for r in rows):
+            return
+    apart(a, (b,), "out[0]")
+
+
+def gated_step(z: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *, starts: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One step of acting: z and x [batch, width], state [batch, width] float32, advanced in place; returns h in z's type.
+    starts: bool [batch], True where the state is not to be used because an episode begins."""
+    need(isinstance(z, torch.Tensor) and isinstance(x, torch.Tensor) and z.dim() == 2 and x.dim() == 2, "z and x are [batch, width]")
+    need(starts is None or starts.dim() == 1, "starts: [batch]")
+    need(state is not None, "state: a float32 tensor [batch, width] to advance")
+    s, dev = _scan(z[:, None], x[:, None], state, None if starts is None else starts[:, None], None)
+    apart(state, (z, x, starts), "state")
+    h = torch.empty(z.shape, dtype=z.dtype, device=dev)
+    if z.numel():
+        with guard(dev):
+            check(lib.rlgan_gated_scan_forward(C.byref(s), SeqRef(h.data_ptr(), s.width, s.width), state.data_ptr(), None, stream_of(dev)),
+                  "rlgan_gated_scan_forward")
+    return h
+
+
+class GatedUnit:
+    """A dense layer of 2 `units` outputs (gates z, then inputs x) followed by the recurrence: the trainable counterpart of
+    `LSTMUnit`.  The layer's parameters and gradients are `gates.canon` and `gates.grad`; the first `units` biases start at
+    `forget_bias`, so that an untrained memory reaches some steps back."""
+
+    def __init__(self, n_in: int, units: int, rng: Optional[np.random.RandomState] = None, kernel: Optional[np.ndarray] = None,
+                 bias: Optional[np.ndarray] = None, forget_bias: float = 2.0):
+        rng = rng or np.random.RandomState()
+        self.n_in, self.units = int(n_in), int(units)
+        if kernel is None:
+            lim = np.sqrt(6.0 / (n_in + 2 * units))
+            kernel = rng.uniform(-lim, lim, (n_in, 2 * units))
+            bias = np.concatenate([np.full(units, forget_bias), np.zeros(units)])
+        self.gates = DenseLayer(self.n_in, 2 * self.units, kernel=kernel, bias=np.asarray(bias).reshape(-1))
+        self._pass = None
+
+    def get_initial_state(self, batch: int) -> torch.Tensor:
+        return torch.zeros((batch, self.units), dtype=torch.float32, device=self.gates.canon.device)
+
+    def _split(self, both: torch.Tensor):
+        return both[..., :self.units], both[..., self.units:]
+
+    def forward(self, x: torch.Tensor, state: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None,
+                lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(h [batch, time, units], state) of float32 inputs [batch, time, n_in]; what `backward` needs is kept."""
+        b, n, _ = x.shape
+        rows = x.reshape(b * n, self.n_in).contiguous()
+        both = self.gates.forward(rows, act=False).view(b, n, 2 * self.units)
+        h, last = gated_scan(*self._split(both), state, starts=starts, lengths=lengths)
+        self._pass = (rows, both, h, state, starts, lengths)
+        return h, last
+
+    def backward(self, dh: torch.Tensor, dstate: Optional[torch.Tensor] = None, need_dx: bool = True):
+        """(dx or None, dstate_in) of the latest `forward`; fills gates.grad."""
+        rows, both, h, state, starts, lengths = self._pass
+        dboth = torch.empty_like(both)
+        _, _, dstate_in = gated_scan_backward(dh, *self._split(both), h, state, starts=starts, lengths=lengths, dstate=dstate,
+                                              out=self._split(dboth))
+        flat = (rows.shape[0], 2 * self.units)
+        dx = self.gates.backward(rows, both.view(flat), dboth.view(flat), need_dx=need_dx, act=False)
+        return (None if dx is None else dx.view(h.shape[0], h.shape[1], self.n_in)), dstate_in
+
+    def step(self, x: torch.Tensor, state: torch.Tensor, starts: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One step of float32 inputs [batch, n_in]; `state` is advanced in place."""
+        return gated_step(*self._split(self.gates.forward(x.contiguous(), act=False)), state, starts=starts)

@@ -1,0 +1,89 @@
+"""What the operators on fp32, bf16 and fp16 tensors share: checks of their arguments, and the device and stream of a call.
+
+Unlike the networks' own buffers, which are fp32 and allocated by this package, these tensors come from a caller, with any row
+strides; a call that a kernel could not take raises ValueError here, before anything is launched."""
+from __future__ import annotations
+
+import contextlib
+from typing import Optional
+
+import torch
+
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # RLGAN_F32, RLGAN_BF16, RLGAN_F16
+
+
+def need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def type_code(t: torch.Tensor, name: str) -> int:
+    code = TYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name} is {t.dtype}: float32, bfloat16 or float16 is wanted")
+    return code
+
+
+def on_device(t: torch.Tensor, dev: torch.device, name: str) -> None:
+    if not t.is_cuda or t.device != dev:
+        raise ValueError(f"{name} is on {t.device}: the call's tensors are on {dev}, an AMD GPU")
+
+
+def first_device(t: torch.Tensor, name: str) -> torch.device:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} has to be a tensor on an AMD GPU (there is no CPU path)")
+    return t.device
+
+
+def vector(t: Optional[torch.Tensor], shape, dev: torch.device, name: str, dtype=torch.float32) -> Optional[int]:
+    """Pointer of a contiguous tensor of that type and shape; None for None."""
+    if t is None:
+        return None
+    on_device(t, dev, name)
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} is wanted, got {t.dtype} {tuple(t.shape)} "
+                         f"with strides {t.stride()}")
+    return t.data_ptr()
+
+
+def byte_range(t: torch.Tensor):
+    """First byte of a tensor and the one behind its last."""
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    return t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def apart(out: torch.Tensor, others, name: str) -> None:
+    """Refuses an output that shares memory with one of `others`, or whose own elements do."""
+    if out.numel() == 0:
+        return
+    lo, hi = byte_range(out)
+    for t in others:
+        if t is not None:
+            a, b = byte_range(t)
+            if a < hi and lo < b:
+                raise ValueError(f"{name} shares memory with another tensor of the call")
+    own_elements(out, name)
+
+
+def own_elements(t: torch.Tensor, name: str) -> None:
+    """Refuses a tensor to be written in which two indices name one element (an expanded one, overlapping windows)."""
+    reach = 1
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if s < reach:
+            raise ValueError(f"{name} has elements that share memory (strides {t.stride()}): it cannot be written")
+        reach = s * (n - 1) + reach
+
+
+def guard(dev: torch.device):
+    """Makes `dev` the current device for the launches of a call."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def stream_of(dev: torch.device) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def workspace(size: int, dev: torch.device) -> Optional[torch.Tensor]:
+    """Scratch memory of one call: allocated for it on the current stream, so that no two calls, streams or graphs share one."""
+    return torch.empty(size, dtype=torch.uint8, device=dev) if size else None
