@@ -4,6 +4,8 @@
 // start), and maps compose: (a2, b2) after (a1, b1) is (a2 a1, a2 b1 + b2).  gfx950 only.
 #include "rlgan_types.h"
 #include "rlgan_host.h"
+#include <algorithm>
+#include <initializer_list>
 
 using namespace rlgan;
 
@@ -101,6 +103,331 @@ __global__ __launch_bounds__(256) void scan_serial_bwd(Units u, Seq<const T> dh,
   for (int k = 0; k < VEC; ++k) dstate_in[(int64_t)b * u.width + d + k] = c[k];
 }
 
+// ---- the tiled form -----------------------------------------------------------------------------------------
+// A workgroup owns 64 * VEC units and walks along time in tiles of WAVES * STEPS steps: each wave takes STEPS consecutive ones,
+// folds them to one affine map, all waves compose the maps before theirs (and, for the next tile, all of them) from LDS, and each
+// then runs its steps again from registers with the right state in front.  Inputs are read once, the next tile's loads are in
+// flight meanwhile, and 8 waves work on units that are one dependent chain.  Where there are too few units to fill the chip the
+// time axis is cut into segments: a first kernel folds every segment to its map, and the walk of a segment begins with the
+// composition of the maps before it.
+
+constexpr int WAVES = 8, STEPS = 8, TILE = WAVES * STEPS;
+
+// h -> a h + b; a < 0 (by its sign bit, which products with f keep): the state from before does not reach through, h -> b
+struct Map { float a, b; };
+__device__ __forceinline__ float apply(Map m, float s) { return __float_as_int(m.a) < 0 ? m.b : m.b + m.a * s; }
+__device__ __forceinline__ Map compose(Map late, Map early) {
+  return {__float_as_int(late.a) < 0 ? late.a : __float_as_int(early.a) < 0 ? early.a : late.a * early.a, apply(late, early.b)};
+}
+constexpr float DROP = -1.f;
+
+template <int VEC> struct Lanes {                // the units of a lane
+  int64_t unit;                                  // first of them, counted through the batch
+  int b, d, len;
+  bool real;
+  __device__ __forceinline__ Lanes(const Units& u, bool mask) {
+    const int wv = u.width / VEC, total = u.batch * wv;
+    const int i = blockIdx.x * 64 + (threadIdx.x & 63), k = min(i, total - 1);   // lanes behind the last repeat it and write nothing
+    real = i < total;
+    b = k / wv; d = (k - b * wv) * VEC;
+    unit = (int64_t)b * u.width + d;
+    len = mask && u.lengths ? min(max(u.lengths[b], 0), u.length) : u.length;
+  }
+};
+
+// STEPS steps from `t0` on of one sequence tensor; steps behind the end of the axis repeat its last one
+template <typename T, int VEC>
+__device__ __forceinline__ void load_steps(Vec<T, VEC> (&v)[STEPS], const T* p, int64_t stride, int t0, int length) {
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) v[i].load(p + min(max(t0 + i, 0), length - 1) * stride);
+}
+__device__ __forceinline__ uint32_t load_starts(const uint8_t* p, int64_t stride, int t0, int length) {
+  uint32_t bits = 0;
+  if (p) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) bits |= (p[min(t0 + i, length - 1) * stride] ? 1u : 0u) << i;
+  }
+  return bits;
+}
+
+// the map of one step, forward: folds it behind m
+__device__ __forceinline__ void fold_forward(Map& m, float f, float take, float x, bool start, bool live) {
+  const float p = start ? 0.f : m.b, b = p + take * (x - p), a = start ? DROP : m.a * f;
+  m = live ? Map{a, b} : m;
+}
+// backward: the gradient that step t hands to the step before it, c' = f (dh + c)
+__device__ __forceinline__ void fold_backward(Map& m, float f, float dh, bool start, bool live) {
+  const float b = start ? 0.f : f * (dh + m.b), a = start ? DROP : m.a * f;
+  m = live ? Map{a, b} : m;
+}
+
+struct Cut { int segment, segments; Map* maps; };    // steps a segment (a multiple of TILE); maps[slot][unit]
+
+// One segment's map.  Forward: slot blockIdx.y + 1 holds segment blockIdx.y, slot 0 the state handed in; backward: slot s of
+// segments + 1 holds segment s (s >= 1), the last one the gradient handed in.
+template <typename T, int VEC, bool MASK, bool BACK>
+__global__ __launch_bounds__(WAVES * 64) void scan_fold_kernel(Units u, Seq<const T> z, Seq<const T> x_or_dh, const float* handed, Cut cut) {
+  __shared__ Map sh[WAVES][64 * VEC];
+  const Lanes<VEC> me(u, MASK);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, seg = BACK ? blockIdx.y + 1 : blockIdx.y;
+  const int64_t units = (int64_t)u.batch * u.width;
+  const int per_wave = cut.segment / WAVES, begin = seg * cut.segment + wave * per_wave, end = min(begin + per_wave, u.length);
+  const T* zp = z.p + me.b * z.b + me.d; const T* xp = x_or_dh.p + me.b * x_or_dh.b + me.d;
+  const uint8_t* sp = MASK && u.starts ? u.starts + me.b * u.starts_b : nullptr;
+  Map m[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) m[k] = {1.f, 0.f};
+  Vec<T, VEC> zv[2][STEPS], xv[2][STEPS];
+  uint32_t st[2] = {0, 0};
+  const int n = end > begin ? (end - begin + STEPS - 1) / STEPS : 0;
+  const int first = BACK ? begin + (n - 1) * STEPS : begin, hop = BACK ? -STEPS : STEPS;
+  if (n > 0) { load_steps(zv[0], zp, z.t, first, u.length); load_steps(xv[0], xp, x_or_dh.t, first, u.length); st[0] = load_starts(sp, u.starts_t, first, u.length); }
+  for (int j = 0; j < n; j += 2) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (j + half >= n) break;
+      const int t0 = first + (j + half) * hop, nt = j + half + 1 < n ? t0 + hop : t0;
+      load_steps(zv[half ^ 1], zp, z.t, nt, u.length); load_steps(xv[half ^ 1], xp, x_or_dh.t, nt, u.length);
+      st[half ^ 1] = load_starts(sp, u.starts_t, nt, u.length);
+#pragma unroll
+      for (int q = 0; q < STEPS; ++q) {
+        const int i = BACK ? STEPS - 1 - q : q, t = t0 + i;
+        const bool start = MASK && ((st[half] >> i) & 1), live = t < (MASK ? min(me.len, end) : end);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          float f, take;
+          gate(zv[half][i].get(k), f, take);
+          if constexpr (BACK) fold_backward(m[k], f, xv[half][i].get(k), start, live);
+          else fold_forward(m[k], f, take, xv[half][i].get(k), start, live);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) sh[wave][lane * VEC + k] = m[k];
+  __syncthreads();
+  if (wave != 0) return;
+  const int slot = BACK ? seg : seg + 1;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    Map all{1.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) all = compose(sh[BACK ? WAVES - 1 - w : w][lane * VEC + k], all);
+    if (!me.real) continue;
+    cut.maps[slot * units + me.unit + k] = all;
+    const int edge = BACK ? cut.segments : 0;            // what the call was handed: it may be overwritten by what it returns
+    if (seg == (BACK ? cut.segments - 1 : 0)) cut.maps[edge * units + me.unit + k] = {DROP, handed ? handed[me.unit + k] : 0.f};
+  }
+}
+
+// state in front of a segment: the maps of all before it, the handed state among them, a share of them to each wave
+template <int VEC, bool BACK>
+__device__ __forceinline__ void enter_segment(const Lanes<VEC>& me, const Cut& cut, int seg, int64_t units, Map (*sh)[64 * VEC], float s[VEC]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lo = BACK ? seg + 1 : 0, count = BACK ? cut.segments - seg : seg + 1, share = (count + WAVES - 1) / WAVES;
+  Map m[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) m[k] = {1.f, 0.f};
+  for (int q = 0; q < share; ++q) {
+    const int j = wave * share + q;
+    if (j >= count) break;
+    const int slot = BACK ? lo + count - 1 - j : lo + j;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) m[k] = compose(cut.maps[slot * units + me.unit + k], m[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) sh[wave][lane * VEC + k] = m[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) v = apply(sh[w][lane * VEC + k], v);
+    s[k] = v;
+  }
+  __syncthreads();
+}
+
+template <typename T, int VEC, bool MASK>
+__global__ __launch_bounds__(WAVES * 64) void scan_walk_fwd(Units u, Seq<const T> z, Seq<const T> x, Seq<T> h, float* state_out, Cut cut) {
+  __shared__ Map sh[2][WAVES][64 * VEC];
+  const Lanes<VEC> me(u, MASK);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, seg = blockIdx.y;
+  const int64_t units = (int64_t)u.batch * u.width;
+  const T* zp = z.p + me.b * z.b + me.d; const T* xp = x.p + me.b * x.b + me.d; T* hp = h.p + me.b * h.b + me.d;
+  const uint8_t* sp = MASK && u.starts ? u.starts + me.b * u.starts_b : nullptr;
+  float s[VEC];
+  const int begin = seg * cut.segment, end = min(begin + cut.segment, u.length);
+  Vec<T, VEC> zn[STEPS], xn[STEPS];
+  load_steps(zn, zp, z.t, begin + wave * STEPS, u.length);
+  load_steps(xn, xp, x.t, begin + wave * STEPS, u.length);
+  uint32_t stn = load_starts(sp, u.starts_t, begin + wave * STEPS, u.length);
+  if (cut.segments > 1) enter_segment<VEC, false>(me, cut, seg, units, sh[0], s);
+  else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) s[k] = u.state ? u.state[me.unit + k] : 0.f;
+  }
+  int turn = 0;
+  for (int tile = begin; tile < end; tile += TILE, turn ^= 1) {
+    const int t0 = tile + wave * STEPS;
+    float take[STEPS][VEC], xf[STEPS][VEC];
+    const uint32_t st = stn;
+    Map m[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) m[k] = {1.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        float f;
+        gate(zn[i].get(k), f, take[i][k]);
+        xf[i][k] = xn[i].get(k);
+        fold_forward(m[k], f, take[i][k], xf[i][k], MASK && ((st >> i) & 1), t0 + i < me.len);
+      }
+    if (tile + TILE < end) {
+      load_steps(zn, zp, z.t, t0 + TILE, u.length);
+      load_steps(xn, xp, x.t, t0 + TILE, u.length);
+      stn = load_starts(sp, u.starts_t, t0 + TILE, u.length);
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sh[turn][wave][lane * VEC + k] = m[k];
+    __syncthreads();
+    float mine[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      float v = s[k];
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        if (w == wave) mine[k] = v;
+        v = apply(sh[turn][w][lane * VEC + k], v);
+      }
+      s[k] = v;
+    }
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      if (t0 + i >= u.length) break;
+      Vec<T, VEC> hv;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const bool live = !MASK || t0 + i < me.len;
+        const float p = MASK && ((st >> i) & 1) ? 0.f : mine[k], v = p + take[i][k] * (xf[i][k] - p);
+        mine[k] = live ? v : mine[k];
+        hv.set(k, live ? v : 0.f);
+      }
+      if (me.real) hv.store(hp + (t0 + i) * h.t);
+    }
+  }
+  if (seg == cut.segments - 1 && wave == 0 && me.real) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) state_out[me.unit + k] = s[k];
+  }
+}
+
+template <typename T, int VEC, bool MASK>
+__global__ __launch_bounds__(WAVES * 64) void scan_walk_bwd(Units u, Seq<const T> dh, Seq<const T> z, Seq<const T> x, Seq<const T> h,
+                                                            const float* dstate, Seq<T> dz, Seq<T> dx, float* dstate_in, Cut cut) {
+  __shared__ Map sh[2][WAVES][64 * VEC];
+  const Lanes<VEC> me(u, MASK);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, seg = blockIdx.y;
+  const int64_t units = (int64_t)u.batch * u.width;
+  const T* gp = dh.p + me.b * dh.b + me.d; const T* zp = z.p + me.b * z.b + me.d;
+  const T* xp = x.p + me.b * x.b + me.d; const T* hp = h.p + me.b * h.b + me.d;
+  T* ozp = dz.p + me.b * dz.b + me.d; T* oxp = dx.p + me.b * dx.b + me.d;
+  const uint8_t* sp = MASK && u.starts ? u.starts + me.b * u.starts_b : nullptr;
+  float c[VEC];
+  const int begin = seg * cut.segment, end = min(begin + cut.segment, u.length);
+  const int last = begin + (end - begin - 1) / TILE * TILE;
+  Vec<T, VEC> zn[STEPS], xn[STEPS], gn[STEPS], hn[STEPS];
+  uint32_t stn;
+  auto fetch = [&](int t0) {
+    load_steps(zn, zp, z.t, t0, u.length);
+    load_steps(gn, gp, dh.t, t0, u.length);
+    load_steps(xn, xp, x.t, t0, u.length);
+    load_steps(hn, hp, h.t, t0 - 1, u.length);
+    stn = load_starts(sp, u.starts_t, t0, u.length);
+  };
+  fetch(last + wave * STEPS);
+  if (cut.segments > 1) enter_segment<VEC, true>(me, cut, seg, units, sh[0], c);
+  else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) c[k] = dstate ? dstate[me.unit + k] : 0.f;
+  }
+  int turn = 0;
+  for (int tile = last; tile >= begin; tile -= TILE, turn ^= 1) {
+    const int t0 = tile + wave * STEPS;
+    float f[STEPS][VEC], take[STEPS][VEC];
+    Vec<T, VEC> xv[STEPS], gv[STEPS], hv[STEPS];
+    const uint32_t st = stn;
+    Map m[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) m[k] = {1.f, 0.f};
+#pragma unroll
+    for (int i = STEPS - 1; i >= 0; --i) {
+      xv[i] = xn[i]; gv[i] = gn[i]; hv[i] = hn[i];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        gate(zn[i].get(k), f[i][k], take[i][k]);
+        fold_backward(m[k], f[i][k], gv[i].get(k), MASK && ((st >> i) & 1), t0 + i < me.len);
+      }
+    }
+    if (tile > begin) fetch(t0 - TILE);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sh[turn][wave][lane * VEC + k] = m[k];
+    __syncthreads();
+    float mine[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      float v = c[k];
+#pragma unroll
+      for (int w = WAVES - 1; w >= 0; --w) {
+        if (w == wave) mine[k] = v;
+        v = apply(sh[turn][w][lane * VEC + k], v);
+      }
+      c[k] = v;
+    }
+#pragma unroll
+    for (int i = STEPS - 1; i >= 0; --i) {
+      if (t0 + i >= u.length) continue;
+      Vec<T, VEC> oz, ox;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const bool live = !MASK || t0 + i < me.len, start = MASK && ((st >> i) & 1);
+        const float before = t0 + i > 0 ? hv[i].get(k) : u.state ? u.state[me.unit + k] : 0.f, p = start ? 0.f : before;
+        const float g = mine[k] + gv[i].get(k), gt = g * take[i][k];
+        ox.set(k, live ? gt : 0.f);
+        oz.set(k, live ? gt * f[i][k] * (p - xv[i].get(k)) : 0.f);
+        mine[k] = live ? (start ? 0.f : f[i][k] * g) : mine[k];
+      }
+      if (me.real) { oz.store(ozp + (t0 + i) * dz.t); ox.store(oxp + (t0 + i) * dx.t); }
+    }
+  }
+  if (seg == 0 && wave == 0 && me.real) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) dstate_in[me.unit + k] = c[k];
+  }
+}
+
+// ---- which form -------------------------------------------------------------------------------------------------
+
+// Up to SERIAL steps one thread a unit is best (a single step is one read and one write); behind that the tiled form.
+constexpr int SERIAL = 8;
+
+struct Plan { bool serial; int vec, tiles; Cut cut; };
+
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// A cut costs a second read of two tensors, idle CUs cost bandwidth.  Measured on an MI355X with 256, 512, 1024, 2048 workgroups
+// wanted: 65536 steps of 512 units forward fp32 161, 145, 149, 154 us, 16385 of 3000 backward bf16 257, 223, 231, 237; and with 256 or
+// more workgroups of units (1024 steps of 32768 units bf16: 46 us) a cut loses (70 us in two segments).
+inline Plan plan(int batch, int length, int width, int vec) {
+  constexpr int WANT = 512;
+  Plan p{length <= SERIAL, vec, (int)cdiv((int64_t)batch * (width / vec), 64), {}};
+  const int64_t segments = p.tiles >= WANT / 2 ? 1 : cdiv(WANT, p.tiles), steps = cdiv(cdiv(length, segments), TILE) * TILE;
+  p.cut.segment = (int)steps;
+  p.cut.segments = (int)cdiv(length, steps);
+  return p;
+}
+
 inline int check_scan(const rlgan_scan_t* s) {
   if (!s || !s->z.p || !s->x.p) return RLGAN_E_ARG;
   if (s->batch <= 0 || s->length <= 0 || s->width <= 0) return RLGAN_E_ARG;
@@ -115,14 +442,43 @@ inline Units units(const rlgan_scan_t* s) {
   return {s->batch, s->length, s->width, s->state, s->starts, s->starts_batch, s->starts_time, s->lengths};
 }
 
+
+// Units a lane takes side by side where the width and every tensor's alignment allow it, else one: 16 bytes of them in the serial
+// form; 4 bytes in the tiled one, where 8 and 16 cost more in registers than wide loads give (1024 steps of 32768 units forward
+// bf16: 46 us with 2 units, 76 with 4, 50 with 1; backward of 25800 units fp32: 40 with 1, 48 with 2).
+inline int vec_of(const rlgan_scan_t* s, std::initializer_list<rlgan_seq_t> seqs) {
+  const int size = s->type == TYPE_F32 ? 4 : 2, vec = (s->length <= SERIAL ? 16 : 4) / size;
+  bool ok = s->width % vec == 0;
+  for (const rlgan_seq_t& q : seqs) ok = ok && (uintptr_t)q.p % (vec * size) == 0 && q.batch % vec == 0 && q.time % vec == 0;
+  return ok ? vec : 1;
+}
+
 }  // namespace
+
+// the statements with the element type T, the mask switch MASK and the units a lane VEC (1 or WIDE / sizeof(T)) of the call
+#define RLGAN_SCAN_VARIANT(WIDE, ...)                                                                             \
+  RLGAN_BY_TYPE(s->type, T, {                                                                                     \
+    if (mask) {                                                                                                   \
+      constexpr bool MASK = true;                                                                                 \
+      if (p.vec == 1) { constexpr int VEC = 1; __VA_ARGS__; } else { constexpr int VEC = WIDE / sizeof(T); __VA_ARGS__; } \
+    } else {                                                                                                      \
+      constexpr bool MASK = false;                                                                                \
+      if (p.vec == 1) { constexpr int VEC = 1; __VA_ARGS__; } else { constexpr int VEC = WIDE / sizeof(T); __VA_ARGS__; } \
+    }                                                                                                             \
+  })
 
 extern "C" {
 
 int rlgan_gated_scan_workspace(int batch, int length, int width, int type, int backward, int64_t* bytes) {
   if (!bytes || batch <= 0 || length <= 0 || width <= 0) return RLGAN_E_ARG;
   if (type < TYPE_F32 || type > TYPE_F16) return RLGAN_E_KIND;
-  *bytes = 0;
+  int64_t most = 0;                              // one or two units a lane: the call decides by its tensors' alignment
+  for (int vec = 1; vec <= 2; ++vec) {
+    if (width % vec) break;
+    const Plan p = plan(batch, length, width, vec);
+    if (!p.serial && p.cut.segments > 1) most = std::max(most, (int64_t)(p.cut.segments + 1) * batch * width * (int64_t)sizeof(Map));
+  }
+  *bytes = most;
   return 0;
 }
 
@@ -131,11 +487,21 @@ int rlgan_gated_scan_forward(const rlgan_scan_t* s, rlgan_seq_t h, float* state_
   if (!h.p || !state_out) return RLGAN_E_ARG;
   const Units u = units(s);
   const bool mask = s->starts || s->lengths;
-  const dim3 grid((unsigned)(((int64_t)s->batch * s->width + 255) / 256));
-  RLGAN_BY_TYPE(s->type, T, {
-    if (mask) hipLaunchKernelGGL((scan_serial_fwd<T, 1, true>), grid, dim3(256), 0, (hipStream_t)stream, u, in<T>(s->z), in<T>(s->x), out<T>(h), state_out);
-    else hipLaunchKernelGGL((scan_serial_fwd<T, 1, false>), grid, dim3(256), 0, (hipStream_t)stream, u, in<T>(s->z), in<T>(s->x), out<T>(h), state_out);
-  });
+  Plan p = plan(s->batch, s->length, s->width, vec_of(s, {s->z, s->x, h}));
+  p.cut.maps = (Map*)workspace;
+  hipStream_t st = (hipStream_t)stream;
+  if (p.serial) {
+    const dim3 grid((unsigned)cdiv((int64_t)s->batch * (s->width / p.vec), 256));
+    RLGAN_SCAN_VARIANT(16, hipLaunchKernelGGL((scan_serial_fwd<T, VEC, MASK>), grid, dim3(256), 0, st, u, in<T>(s->z), in<T>(s->x), out<T>(h), state_out));
+    return (int)hipGetLastError();
+  }
+  if (p.cut.segments > 1) {
+    if (!workspace) return RLGAN_E_ARG;
+    RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_fold_kernel<T, VEC, MASK, false>), dim3(p.tiles, p.cut.segments - 1), dim3(WAVES * 64), 0, st, u,
+                                          in<T>(s->z), in<T>(s->x), s->state, p.cut));
+  }
+  RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_walk_fwd<T, VEC, MASK>), dim3(p.tiles, p.cut.segments), dim3(WAVES * 64), 0, st, u, in<T>(s->z),
+                                        in<T>(s->x), out<T>(h), state_out, p.cut));
   return (int)hipGetLastError();
 }
 
@@ -145,11 +511,22 @@ int rlgan_gated_scan_backward(const rlgan_scan_t* s, rlgan_seq_t h, rlgan_seq_t 
   if (!h.p || !dh.p || !dz.p || !dx.p || !dstate_in) return RLGAN_E_ARG;
   const Units u = units(s);
   const bool mask = s->starts || s->lengths;
-  const dim3 grid((unsigned)(((int64_t)s->batch * s->width + 255) / 256));
-  RLGAN_BY_TYPE(s->type, T, {
-    if (mask) hipLaunchKernelGGL((scan_serial_bwd<T, 1, true>), grid, dim3(256), 0, (hipStream_t)stream, u, in<T>(dh), in<T>(s->z), in<T>(s->x), in<T>(h), dstate, out<T>(dz), out<T>(dx), dstate_in);
-    else hipLaunchKernelGGL((scan_serial_bwd<T, 1, false>), grid, dim3(256), 0, (hipStream_t)stream, u, in<T>(dh), in<T>(s->z), in<T>(s->x), in<T>(h), dstate, out<T>(dz), out<T>(dx), dstate_in);
-  });
+  Plan p = plan(s->batch, s->length, s->width, vec_of(s, {s->z, s->x, h, dh, dz, dx}));
+  p.cut.maps = (Map*)workspace;
+  hipStream_t st = (hipStream_t)stream;
+  if (p.serial) {
+    const dim3 grid((unsigned)cdiv((int64_t)s->batch * (s->width / p.vec), 256));
+    RLGAN_SCAN_VARIANT(16, hipLaunchKernelGGL((scan_serial_bwd<T, VEC, MASK>), grid, dim3(256), 0, st, u, in<T>(dh), in<T>(s->z), in<T>(s->x), in<T>(h),
+                                          dstate, out<T>(dz), out<T>(dx), dstate_in));
+    return (int)hipGetLastError();
+  }
+  if (p.cut.segments > 1) {
+    if (!workspace) return RLGAN_E_ARG;
+    RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_fold_kernel<T, VEC, MASK, true>), dim3(p.tiles, p.cut.segments - 1), dim3(WAVES * 64), 0, st, u,
+                                          in<T>(s->z), in<T>(dh), dstate, p.cut));
+  }
+  RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_walk_bwd<T, VEC, MASK>), dim3(p.tiles, p.cut.segments), dim3(WAVES * 64), 0, st, u, in<T>(dh),
+                                        in<T>(s->z), in<T>(s->x), in<T>(h), dstate, out<T>(dz), out<T>(dx), dstate_in, p.cut));
   return (int)hipGetLastError();
 }
 

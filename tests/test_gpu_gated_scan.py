@@ -129,7 +129,10 @@ def test_extreme_gates():
         s["z"][:, 3::7], s["z"][:, 5::11], s["z"][0, 8], s["z"][1, 9] = big, -big, float("inf"), float("-inf")
         h = _check(s, kind)[0]
         assert torch.isfinite(h).all()
-        assert torch.equal(h[0, 8], h[0, 7])
+        # with f = 1 the state stays: both steps hold the same exact value, each within the bound above of it (the second one may
+        # begin a span, whose state comes from the maps before it), and for 16 bits they may round to neighbours
+        top = max(1.0, float(h.abs().max()))
+        assert (h[0, 8].float() - h[0, 7].float()).abs().max() <= (2 * (13 * 40 + 32) * U + torch.finfo(t).eps) * top
 
 
 @pytest.mark.parametrize("n", [40, 3000])
