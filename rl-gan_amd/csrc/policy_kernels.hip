@@ -6,6 +6,7 @@
 // gfx950 only.
 #include "rlgan_types.h"
 #include "rlgan_host.h"
+#include <algorithm>
 
 using namespace rlgan;
 
@@ -20,140 +21,526 @@ struct Policy {
   const void* actions; int action64;
   const float* old_logp; const float* advantages; const float* weights; const float* ref_logp;
   const uint8_t* legal;
-  float scale2;                       // log2(e) / tau: a difference of logits in the exponent of 2
+  float scale;                        // log2(e) / tau: a difference of logits in the exponent of 2
   double inv_tau, low, high, beta, eta, row_weight;
-  float* logp; float* entropy; float* kl; double* row_loss;
+  float* logp; float* entropy; float* kl;
 };
 
-// what the gradient of a row is made of: d_j = e_j (a0 + a1 x2_j) with e_j = 2^(x2_j - log2_s), and `at` more at the action
-struct RowGrad { float log2_s, a0, a1, at; int64_t action; };
+// what the gradient of a row is made of: d_j = 2^y_j (a0 + a1 y_j) with y_j = z_j scale - shift = log2 p_j, and `at` more at the action
+struct RowGrad { float shift, a0, a1, at; int action; };
 
-template <typename T> __device__ __forceinline__ bool in_row(const Policy& P, const T* z, const uint8_t* legal, int j) {
-  return !legal || legal[j];
+// What a row comes with, read ahead of its logits' sums by the thread that will finish it.
+struct RowIn { int64_t action; float z_action, weight, advantage, old_logp, ref_logp; bool legal; };
+
+template <typename T> __device__ __forceinline__ float logit_of(const Policy& P, const T* z, int64_t a) {
+  return a >= 0 && a < P.vocab ? (float)z[a] : 0.f;
+}
+__device__ __forceinline__ RowIn row_in(const Policy& P, int64_t row) {
+  RowIn r;
+  r.action = P.action64 ? ((const int64_t*)P.actions)[row] : (int64_t)((const int32_t*)P.actions)[row];
+  r.weight = P.weights ? P.weights[row] : 1.f;
+  r.advantage = P.advantages[row];
+  r.old_logp = P.old_logp[row];
+  r.ref_logp = P.ref_logp ? P.ref_logp[row] : 0.f;
+  r.legal = !P.legal || r.action < 0 || r.action >= P.vocab || P.legal[row * P.ld_legal + r.action];
+  return r;
 }
 
-// A row's numbers from its maximum, sum and weighted sum (x in units of log 2).  In 64 bits: the terms cancel against each other
-// and a batch's rows do too, and one lane of a row does this once.  `writer`: the thread that leaves the row's results.
+// maximum m, sum s of 2^x and t of x 2^x with x = z scale - shift(m), of some of a row's logits.  NaN logits show in s; x is held
+// above -1e4 where it is a factor, so that what has no weight (-inf) adds 0 and not 0 * inf.
+struct Stats { float m, s, t; };
+
+// What 2's exponent of a row's maximum is: x = z scale - shift rounds once, and as shift is the same for the whole row its own
+// rounding drops out of every probability (finish_row uses it as it is).  Beyond FAR the product would overflow; there one step of
+// the type is so large that a logit is the maximum or has no weight: `settle` makes that so, and the shift is 0.
+constexpr float FAR = 1e37f;
+__device__ __forceinline__ bool is_far(float m, float scale) { return m != -INFINITY && !(fabsf(m * scale) < FAR); }
+__device__ __forceinline__ float shift_of(float m, float scale) { return m == -INFINITY || is_far(m, scale) ? 0.f : m * scale; }
+// a far logit with its maximum taken away
+__device__ __forceinline__ float settled(float z, float m) {
+  const float d = z - m;
+  return d == 0.f ? 0.f : d < 0.f ? -INFINITY : __builtin_nanf("");
+}
+
+// A row's results from its sums.  In 64 bits: the terms cancel against each other and a batch's rows do too, and one lane of a row
+// does this once.  `writer`: the thread that leaves the row's results; loss: the row's weighted share.
 // Rows left out (action < 0, weight 0, an action that is not allowed): zeros everywhere.  An action >= vocab: NaN everywhere.
-template <typename T>
-__device__ RowGrad finish_row(const Policy& P, const T* z, int64_t row, float top, float s, float t2, bool writer) {
-  const int64_t a = P.action64 ? ((const int64_t*)P.actions)[row] : ((const int32_t*)P.actions)[row];
-  const double w = P.weights ? (double)P.weights[row] : P.row_weight;
+__device__ RowGrad finish_row(const Policy& P, int64_t row, const RowIn& in, const Stats& st, bool writer, double& loss) {
+  const double w = P.weights ? (double)in.weight : P.row_weight;
   RowGrad g{0.f, 0.f, 0.f, 0.f, -1};
-  double loss = 0, logp = 0, entropy = 0, kl = 0;
-  bool used = a >= 0 && w != 0;
-  if (used && a >= P.vocab) {
+  double logp = 0, entropy = 0, kl = 0;
+  loss = 0;
+  bool used = in.action >= 0 && w != 0;
+  if (used && in.action >= P.vocab) {
     used = false;
     const float nan = __builtin_nanf("");
     loss = logp = entropy = kl = nan;
     g.a0 = nan;
   }
-  if (used && P.legal && !P.legal[row * P.ld_legal + a]) used = false;
-  float za = 0.f;
+  used = used && in.legal && in.z_action != -INFINITY;
   if (used) {
-    za = (float)z[a];
-    if (za == -INFINITY) used = false;
-  }
-  if (used) {
-    const double adv = P.advantages[row], log_s = log((double)s);
-    logp = ((double)za - (double)top) * P.inv_tau - log_s;
-    entropy = log_s - LN2 * (double)t2 / (double)s;
-    const double r = exp(logp - (double)P.old_logp[row]), lo = 1 - P.low, hi = 1 + P.high;
+    const double adv = in.advantage, log_s = log((double)st.s);
+    const float za = is_far(st.m, P.scale) ? settled(in.z_action, st.m) : in.z_action, shift = shift_of(st.m, P.scale);
+    logp = LN2 * ((double)za * (double)P.scale - (double)shift) - log_s;
+    entropy = log_s - LN2 * (double)st.t / (double)st.s;
+    const double r = exp(logp - (double)in.old_logp), lo = 1 - P.low, hi = 1 + P.high;
     const double held = (r < lo ? lo : r > hi ? hi : r) * adv, free = r * adv;
     const bool clipped = free > held;                        // a NaN is never clipped away
     double slope = clipped ? 0.0 : -free;
     loss = -(clipped ? held : free) - P.eta * entropy;
     if (P.ref_logp) {
-      const double d = (double)P.ref_logp[row] - logp, em = expm1(d);
+      const double d = (double)in.ref_logp - logp, em = expm1(d);
       kl = em - d;
       loss += P.beta * kl;
       slope -= P.beta * em;
     }
     loss *= w;
     const double k = w * P.inv_tau;
-    g.log2_s = (float)(log_s * (double)LOG2E);
-    g.a0 = (float)(k * (P.eta * (entropy - log_s) - slope));
+    g.shift = (float)((double)shift + log_s * (double)LOG2E);
+    g.a0 = (float)(k * (P.eta * entropy - slope));
     g.a1 = (float)(k * P.eta * LN2);
     g.at = (float)(k * slope);
-    g.action = a;
+    g.action = (int)in.action;
   }
-  if (writer) {
-    P.logp[row] = (float)logp; P.entropy[row] = (float)entropy; P.kl[row] = (float)kl;
-    P.row_loss[row] = loss;
-  }
+  if (writer) { P.logp[row] = (float)logp; P.entropy[row] = (float)entropy; P.kl[row] = (float)kl; }
   return g;
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) { const float u = __shfl_xor(v, o); v = u > v || u != u ? u : v; }
-  return v;
+// a value that is the same in all lanes of a wave, as a scalar
+__device__ __forceinline__ float uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
+__device__ __forceinline__ RowGrad uniform(const RowGrad& g) {
+  return {uniform(g.shift), uniform(g.a0), uniform(g.a1), uniform(g.at), __builtin_amdgcn_readfirstlane(g.action)};
 }
 
-// a workgroup a row, the row read three times
-template <typename T, bool GRAD>
-__global__ __launch_bounds__(256) void policy_rows_kernel(Policy P, const T* logits, T* dlogits) {
-  __shared__ float sh[8];
-  __shared__ RowGrad shared_row;
-  const int64_t row = blockIdx.x;
-  const T* z = logits + row * P.ld;
-  const uint8_t* legal = P.legal ? P.legal + row * P.ld_legal : nullptr;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float top = -INFINITY;
-  for (int j = threadIdx.x; j < P.vocab; j += 256) {
-    const float v = in_row(P, z, legal, j) ? (float)z[j] : -INFINITY;
-    top = v > top || v != v ? v : top;
+// the same with another maximum
+__device__ __forceinline__ Stats moved(Stats a, float m, float scale) {
+  const float d0 = is_far(m, scale) || is_far(a.m, scale) ? settled(a.m, m) : a.m == -INFINITY ? -INFINITY : shift_of(a.m, scale) - shift_of(m, scale);
+  const float d = a.m == m ? 0.f : fmaxf(d0, -1e4f), e = __builtin_amdgcn_exp2f(d);
+  return {m, a.s * e, (a.t + d * a.s) * e};
+}
+// over GROUP neighbouring lanes; the same bits in all of them
+template <int GROUP> __device__ __forceinline__ Stats merge_lanes(Stats a, float scale) {
+#pragma unroll
+  for (int o = GROUP / 2; o > 0; o >>= 1) {
+    const Stats b{__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.t, o)};
+    const float m = fmaxf(a.m, b.m);
+    const Stats u = moved(a, m, scale), v = moved(b, m, scale);
+    a = {m, u.s + v.s, u.t + v.t};
   }
-  top = wave_max(top);
-  if (lane == 0) sh[wave] = top;
-  __syncthreads();
-  top = sh[0];
-  for (int w = 1; w < 4; ++w) top = sh[w] > top || sh[w] != sh[w] ? sh[w] : top;
-  if (top == -INFINITY) top = 0.f;
-  __syncthreads();
-  float s = 0.f, t2 = 0.f;
-  for (int j = threadIdx.x; j < P.vocab; j += 256) {
-    const float v = in_row(P, z, legal, j) ? (float)z[j] : -INFINITY, x2 = (v - top) * P.scale2, e = __builtin_amdgcn_exp2f(x2);
-    s += e;
-    t2 += fmaxf(x2, -1e4f) * e;
+  return a;
+}
+
+// A row's columns are counted from `skew` elements before its first, where a 16-byte vector begins in memory (0 for rows whose
+// vectors are no such ones): loads and stores are then aligned whatever the leading dimension, but for a row's first and last.
+template <typename T, int N> __device__ __forceinline__ int skew_of(const T* z) {
+  return N * sizeof(T) == 16 ? (int)(((uintptr_t)z / sizeof(T)) % N) : 0;
+}
+// first column that a vector at column j reads: the row's first and last vectors are moved inside (a row has at least N)
+template <int N> __device__ __forceinline__ int inside(const Policy& P, int j) { return min(max(j, 0), P.vocab - N); }
+
+// N logits for columns j .. j + N - 1, -inf where there is none or it is not legal
+template <typename T, int N>
+__device__ __forceinline__ void load_logits(const Policy& P, const T* z, const uint8_t* legal, int j, Words<T, N>& v) {
+  const int at = inside<N>(P, j);
+  v.load(z + at);
+  Vec<uint8_t, N> ok;
+  if (legal) ok.load(legal + at);
+  if (at != j) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) if (at + i < j || at + i >= j + N) v.set_infinite(i);
   }
-  s = wave_sum(s); t2 = wave_sum(t2);
-  if (lane == 0) { sh[wave] = s; sh[4 + wave] = t2; }
+  if (legal) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) if (!ok.v[i]) v.set_infinite(i);
+  }
+}
+
+template <typename T, int N> __device__ __forceinline__ float max_of(const Words<T, N>& v, float m) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = fmaxf(m, v.get(i));
+  return m;
+}
+template <typename T, int N> __device__ __forceinline__ void settle(Words<T, N>& v, float m) {
+  float d[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) d[i] = settled(v.get(i), m);
+  v.set_all(d);
+}
+template <typename T, int N> __device__ __forceinline__ void add_to(Stats& a, const Words<T, N>& v, float shift, float scale) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float x = __builtin_fmaf(v.get(i), scale, -shift), e = __builtin_amdgcn_exp2f(x);
+    a.s += e;
+    a.t += fmaxf(x, -1e4f) * e;
+  }
+}
+
+// gradients for columns j .. j + N - 1, written to d (the row's)
+template <typename T, int N>
+__device__ __forceinline__ void write_grad(const Policy& P, const Words<T, N>& v, int j, const RowGrad& g, T* d) {
+  if (j >= P.vocab) return;
+  Words<T, N> out;
+  float val[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float y = __builtin_fmaf(v.get(i), P.scale, -g.shift);
+    val[i] = __builtin_amdgcn_exp2f(y) * (g.a0 + g.a1 * fmaxf(y, -1e4f));
+  }
+  const int at = inside<N>(P, j);
+  if (g.action < 0) {                                    // a row left out: zeros; no such action: NaN
+#pragma unroll
+    for (int i = 0; i < N; ++i) val[i] = g.a0;
+  } else if (g.action >= at && g.action < at + N) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) if (at + i == g.action) val[i] += g.at;
+  }
+  out.set_all(val);
+  if (at == j) out.store(d + j);
+  else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) if (at + i >= j && at + i < j + N) d[at + i] = out.element(i);
+  }
+}
+
+// ---- rows that fit the registers of their threads -------------------------------------------------------------------
+// GROUP threads hold K rows, each in C vectors of N a thread: read once, written once.  A row's sums are joined by shuffles (and
+// through LDS where it has several waves); then one thread a row finishes it, those of a workgroup side by side: with a row a
+// wave and K = 1 the 64-bit arithmetic of a single lane took more time than the row's memory.  parts: one sum of row losses a
+// workgroup.
+template <typename T, int N, int C, int GROUP, int K, bool GRAD>
+__global__ __launch_bounds__(GROUP > 256 ? GROUP : 256, N * C * K * sizeof(T) > 128 ? 4 : K > 1 || N * C * K * sizeof(T) > 64 ? 5 : 6)
+void policy_held_kernel(Policy P, const T* logits, T* dlogits, double* parts) {
+  constexpr int THREADS = GROUP > 256 ? GROUP : 256, ROWS = THREADS / GROUP * K, WAVES = GROUP > 64 ? GROUP / 64 : 1;
+  static_assert(WAVES == 1 || K == 1, "a row of several waves is alone in its workgroup");
+  static_assert(ROWS <= THREADS, "a thread finishes one row");
+  __shared__ Stats sh[ROWS * WAVES];
+  __shared__ RowGrad sh_row[ROWS];
+  __shared__ double sh_loss[4];
+  const int me = threadIdx.x % GROUP, slot = threadIdx.x / GROUP * K;
+  const int64_t row0 = (int64_t)blockIdx.x * ROWS;
+  const int wave0 = (GROUP >= 64 ? me & ~63 : 0) * N;                // first column of the wave's first vector
+  Words<T, N> v[K][C];
+  int skew[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int64_t row = min(row0 + slot + k, P.rows - 1);            // behind the last row: the last again, not written
+    const T* z = logits + row * P.ld;
+    skew[k] = skew_of<T, N>(z);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (c * GROUP * N + wave0 < P.vocab + skew[k])
+        load_logits<T, N>(P, z, P.legal ? P.legal + row * P.ld_legal : nullptr, (c * GROUP + me) * N - skew[k], v[k][c]);
+  }
+  const int64_t my_row = row0 + threadIdx.x;                          // the row that this thread finishes
+  const bool mine = threadIdx.x < ROWS && my_row < P.rows;
+  constexpr bool AHEAD = GROUP <= 256;                                // (more threads have no registers left for it)
+  RowIn in;
+  if (AHEAD && mine) {
+    in = row_in(P, my_row);
+    in.z_action = logit_of(P, logits + my_row * P.ld, in.action);
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    Stats st{-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (c * GROUP * N + wave0 < P.vocab + skew[k]) { st.m = max_of(v[k][c], st.m); v[k][c].pin(); }
+    if constexpr (GROUP <= 64) {
+#pragma unroll
+      for (int o = GROUP / 2; o > 0; o >>= 1) st.m = fmaxf(st.m, __shfl_xor(st.m, o));
+    } else {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) st.m = fmaxf(st.m, __shfl_xor(st.m, o));
+      if ((threadIdx.x & 63) == 0) sh[me / 64].m = st.m;
+      __syncthreads();
+#pragma unroll 4
+      for (int w = 0; w < WAVES; ++w) st.m = fmaxf(st.m, sh[w].m);
+      st.m = uniform(st.m);
+    }
+    if (is_far(st.m, P.scale)) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (c * GROUP * N + wave0 < P.vocab + skew[k]) settle(v[k][c], st.m);
+    }
+    const float shift = shift_of(st.m, P.scale);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (c * GROUP * N + wave0 < P.vocab + skew[k]) { add_to(st, v[k][c], shift, P.scale); v[k][c].pin(); }
+#pragma unroll
+    for (int o = (GROUP < 64 ? GROUP : 64) / 2; o > 0; o >>= 1) { st.s += __shfl_xor(st.s, o); st.t += __shfl_xor(st.t, o); }
+    if constexpr (WAVES > 1) __syncthreads();                         // the maxima have been read
+    if ((WAVES > 1 ? threadIdx.x & 63 : me) == 0) sh[WAVES > 1 ? me / 64 : slot + k] = st;
+  }
   __syncthreads();
-  s = sh[0] + sh[1] + sh[2] + sh[3]; t2 = sh[4] + sh[5] + sh[6] + sh[7];
-  if (threadIdx.x == 0) shared_row = finish_row(P, z, row, top, s, t2, true);
+  double loss = 0;
+  if (mine) {
+    if (!AHEAD) {
+      in = row_in(P, my_row);
+      in.z_action = logit_of(P, logits + my_row * P.ld, in.action);
+    }
+    Stats st = sh[threadIdx.x * WAVES];
+#pragma unroll 4
+    for (int w = 1; w < WAVES; ++w) { st.s += sh[w].s; st.t += sh[w].t; }
+    sh_row[threadIdx.x] = finish_row(P, my_row, in, st, true, loss);
+  }
+  if (threadIdx.x < 256) {
+    if constexpr (ROWS > 1) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) loss += __shfl_xor(loss, o);
+    }
+    if ((threadIdx.x & 63) == 0) sh_loss[threadIdx.x >> 6] = loss;
+  }
   __syncthreads();
+  if (threadIdx.x == 0) parts[blockIdx.x] = ((sh_loss[0] + sh_loss[1]) + sh_loss[2]) + sh_loss[3];
   if constexpr (GRAD) {
-    const RowGrad g = shared_row;
-    T* d = dlogits + row * P.ld_d;
-    for (int j = threadIdx.x; j < P.vocab; j += 256) {
-      float v = g.a0;
-      if (g.action >= 0) {
-        const float zj = in_row(P, z, legal, j) ? (float)z[j] : -INFINITY, x2 = (zj - top) * P.scale2;
-        v = __builtin_amdgcn_exp2f(x2 - g.log2_s) * (g.a0 + g.a1 * fmaxf(x2, -1e4f));
-        if (j == g.action) v += g.at;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (row0 + slot + k >= P.rows) break;
+      const RowGrad g = GROUP >= 64 ? uniform(sh_row[slot + k]) : sh_row[slot + k];
+      T* d = dlogits + (row0 + slot + k) * P.ld_d;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        if (c * GROUP * N + wave0 < P.vocab + skew[k]) write_grad<T, N>(P, v[k][c], (c * GROUP + me) * N - skew[k], g, d);
+        __builtin_amdgcn_sched_barrier(0);                 // vector by vector: side by side they would not fit the registers
       }
-      d[j] = (T)v;
     }
   }
 }
 
-__global__ __launch_bounds__(1024) void policy_sum_kernel(const double* parts, int64_t n, float* loss) {
-  __shared__ double sh[1024];
-  double s = 0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) s += parts[i];
-  sh[threadIdx.x] = s;
-  __syncthreads();
-  for (int o = 512; o > 0; o >>= 1) {
-    if ((int)threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
-    __syncthreads();
+// ---- rows that are swept ------------------------------------------------------------------------------------------------
+// Wider rows, rows without a gradient to write, and rows that several workgroups share: a sweep over some of a row's columns keeps
+// a running maximum and moves the sums when it grows; the gradient's sweep reads them again, from the caches.
+constexpr int SWEEP = 512, UNROLL = 4;
+
+// columns begin - skew .. end - skew of a row (its last ones in the piece that reaches vocab + skew)
+template <typename T, int N>
+__device__ Stats sweep_stats(const Policy& P, const T* z, const uint8_t* legal, int skew, int begin, int end) {
+  Stats st{-INFINITY, 0.f, 0.f};
+  for (int j0 = begin; j0 < end; j0 += SWEEP * N * UNROLL) {
+    Words<T, N> v[UNROLL];
+    float m = st.m;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (j0 + u * SWEEP * N < end) load_logits<T, N>(P, z, legal, j0 + (u * SWEEP + (int)threadIdx.x) * N - skew, v[u]);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (j0 + u * SWEEP * N < end) { m = max_of(v[u], m); v[u].pin(); }
+    st = moved(st, m, P.scale);
+    const float shift = shift_of(m, P.scale);
+    if (is_far(m, P.scale)) {
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u)
+        if (j0 + u * SWEEP * N < end) settle(v[u], m);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (j0 + u * SWEEP * N < end) add_to(st, v[u], shift, P.scale);
   }
-  if (threadIdx.x == 0) *loss = (float)sh[0];
+  return st;
+}
+
+template <typename T, int N>
+__device__ void sweep_grad(const Policy& P, const T* z, const uint8_t* legal, int skew, int begin, int end, float top, const RowGrad& g, T* d) {
+  const bool far = is_far(top, P.scale);
+  for (int j0 = begin; j0 < end; j0 += SWEEP * N * UNROLL) {
+    Words<T, N> v[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (j0 + u * SWEEP * N < end) load_logits<T, N>(P, z, legal, j0 + (u * SWEEP + (int)threadIdx.x) * N - skew, v[u]);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (j0 + u * SWEEP * N < end) {
+        if (far) settle(v[u], top);
+        write_grad<T, N>(P, v[u], j0 + (u * SWEEP + (int)threadIdx.x) * N - skew, g, d);
+      }
+  }
+}
+
+// the workgroup's statistics, in its first wave
+__device__ __forceinline__ Stats merge_block(Stats st, Stats* sh, float scale) {
+  st = merge_lanes<64>(st, scale);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = st;
+  __syncthreads();
+  return threadIdx.x < 64 ? merge_lanes<SWEEP / 64>(sh[threadIdx.x % (SWEEP / 64)], scale) : st;
+}
+
+// a row a workgroup
+template <typename T, int N, bool GRAD>
+__global__ __launch_bounds__(SWEEP) void policy_swept_kernel(Policy P, const T* logits, T* dlogits, double* parts) {
+  __shared__ Stats sh[SWEEP / 64];
+  __shared__ RowGrad sh_row;
+  __shared__ float sh_top;
+  const int64_t row = blockIdx.x;
+  const T* z = logits + row * P.ld;
+  const uint8_t* legal = P.legal ? P.legal + row * P.ld_legal : nullptr;
+  const int skew = skew_of<T, N>(z);
+  RowIn in;
+  if (threadIdx.x == 0) {
+    in = row_in(P, row);
+    in.z_action = logit_of(P, z, in.action);
+  }
+  const Stats st = merge_block(sweep_stats<T, N>(P, z, legal, skew, 0, P.vocab + skew), sh, P.scale);
+  if (threadIdx.x == 0) {
+    sh_top = st.m;
+    sh_row = finish_row(P, row, in, st, true, parts[row]);
+  }
+  if constexpr (GRAD) {
+    __syncthreads();
+    sweep_grad<T, N>(P, z, legal, skew, 0, P.vocab + skew, uniform(sh_top), uniform(sh_row), dlogits + row * P.ld_d);
+  }
+}
+
+// several workgroups a row, each on `piece` columns: first their statistics, then (the row's joined by each for itself) the gradient
+template <typename T, int N>
+__global__ __launch_bounds__(SWEEP) void policy_piece_kernel(Policy P, const T* logits, int piece, Stats* pieces, float* z_action) {
+  __shared__ Stats sh[SWEEP / 64];
+  const int64_t row = blockIdx.y;
+  const T* z = logits + row * P.ld;
+  const int skew = skew_of<T, N>(z), begin = blockIdx.x * piece;
+  const Stats st = merge_block(sweep_stats<T, N>(P, z, P.legal ? P.legal + row * P.ld_legal : nullptr, skew, begin,
+                                                 min(begin + piece, P.vocab + skew)), sh, P.scale);
+  if (threadIdx.x == 0) {
+    pieces[row * gridDim.x + blockIdx.x] = st;
+    if (blockIdx.x == 0) z_action[row] = logit_of(P, z, row_in(P, row).action);       // the gradient may overwrite the logits
+  }
+}
+template <typename T, int N, bool GRAD>
+__global__ __launch_bounds__(SWEEP) void policy_join_kernel(Policy P, const T* logits, T* dlogits, int piece, int cuts, const Stats* pieces,
+                                                            const float* z_action, double* parts) {
+  __shared__ RowGrad sh_row;
+  __shared__ float sh_top;
+  const int64_t row = blockIdx.y;
+  if (threadIdx.x < 64) {                                    // at most 64 cuts
+    RowIn in;
+    if (threadIdx.x == 0) {
+      in = row_in(P, row);
+      in.z_action = z_action[row];
+    }
+    Stats st{-INFINITY, 0.f, 0.f};
+    if ((int)threadIdx.x < cuts) st = pieces[row * cuts + threadIdx.x];
+    st = merge_lanes<64>(st, P.scale);
+    if (threadIdx.x == 0) {
+      double loss;
+      sh_top = st.m;
+      sh_row = finish_row(P, row, in, st, blockIdx.x == 0, loss);
+      if (blockIdx.x == 0) parts[row] = loss;
+    }
+  }
+  if constexpr (GRAD) {
+    __syncthreads();
+    const T* z = logits + row * P.ld;
+    const int skew = skew_of<T, N>(z), begin = blockIdx.x * piece;
+    sweep_grad<T, N>(P, z, P.legal ? P.legal + row * P.ld_legal : nullptr, skew, begin, min(begin + piece, P.vocab + skew), uniform(sh_top),
+                     uniform(sh_row), dlogits + row * P.ld_d);
+  }
+}
+
+__global__ __launch_bounds__(1024) void policy_sum_kernel(const double* parts, int64_t n, float* loss) {
+  __shared__ double sh[16];
+  double s = 0;
+  for (int64_t i0 = 0; i0 < n; i0 += 8192) {
+    double v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int64_t i = i0 + k * 1024 + threadIdx.x;
+      v[k] = i < n ? parts[i] : 0.0;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += v[k];
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) s += sh[w];
+    *loss = (float)s;
+  }
+}
+
+// ---- which form -----------------------------------------------------------------------------------------------------------
+
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+constexpr int MAX_CUTS = 64;
+
+struct Cuts { int count, piece; };
+inline Cuts cuts_of(int64_t rows, int vocab, int type) {
+  constexpr int WANT = 512;
+  const int n = type == TYPE_F32 ? 4 : 8, step = SWEEP * n, columns = vocab + n - 1;      // step: a vector of every thread; n - 1: the skew
+  if (rows >= WANT / 2 || vocab <= step) return {1, vocab};
+  const int64_t count = std::min<int64_t>(std::min<int64_t>(cdiv(WANT, rows), cdiv(columns, step)), MAX_CUTS);
+  const int piece = (int)(cdiv(cdiv(columns, count), step) * step);
+  return {(int)cdiv(columns, piece), piece};
+}
+
+template <typename T, int N, int C, int GROUP, int K>
+void launch_held(const Policy& P, const rlgan_policy_t* p, double* parts, int64_t* n_parts, hipStream_t st) {
+  constexpr int THREADS = GROUP > 256 ? GROUP : 256, ROWS = THREADS / GROUP * K;
+  if constexpr (K > 1) {                                                 // few rows: every group takes one
+    if (cdiv(p->rows, ROWS) < 512) return launch_held<T, N, C, GROUP, 1>(P, p, parts, n_parts, st);
+  }
+  *n_parts = cdiv(p->rows, ROWS);
+  if (p->dlogits)
+    hipLaunchKernelGGL((policy_held_kernel<T, N, C, GROUP, K, true>), dim3((unsigned)*n_parts), dim3(THREADS), 0, st, P, (const T*)p->logits,
+                       (T*)p->dlogits, parts);
+  else
+    hipLaunchKernelGGL((policy_held_kernel<T, N, C, GROUP, K, false>), dim3((unsigned)*n_parts), dim3(THREADS), 0, st, P, (const T*)p->logits,
+                       (T*)nullptr, parts);
+}
+
+template <typename T>
+void launch_rows(const Policy& P, const rlgan_policy_t* p, void* workspace, int64_t* n_parts, hipStream_t st) {
+  constexpr int W = 16 / sizeof(T);                                      // elements of a 16-byte vector
+  const int64_t rows = p->rows, vocab = p->vocab;
+  double* parts = (double*)workspace;
+  const Cuts cut = cuts_of(rows, p->vocab, p->type);
+  if (cut.count > 1) {
+    Stats* pieces = (Stats*)(parts + rows);
+    float* za = (float*)(pieces + rows * cut.count);
+    *n_parts = rows;
+    hipLaunchKernelGGL((policy_piece_kernel<T, W>), dim3(cut.count, (unsigned)rows), dim3(SWEEP), 0, st, P, (const T*)p->logits, cut.piece, pieces, za);
+    if (p->dlogits)
+      hipLaunchKernelGGL((policy_join_kernel<T, W, true>), dim3(cut.count, (unsigned)rows), dim3(SWEEP), 0, st, P, (const T*)p->logits,
+                         (T*)p->dlogits, cut.piece, cut.count, pieces, za, parts);
+    else
+      hipLaunchKernelGGL((policy_join_kernel<T, W, false>), dim3(1, (unsigned)rows), dim3(SWEEP), 0, st, P, (const T*)p->logits, (T*)nullptr,
+                         cut.piece, cut.count, pieces, za, parts);
+    return;
+  }
+#define HELD(N, C, GROUP, K) return launch_held<T, N, C, GROUP, K>(P, p, parts, n_parts, st)
+  constexpr int V = sizeof(T) == 4 ? 2 : 4;
+  // room for the skew of rows that begin anywhere
+  const bool aligned = (uintptr_t)p->logits % 16 == 0 && (rows == 1 || p->ld % W == 0);
+  const int64_t columns = vocab + (aligned ? 0 : W - 1), narrow = W == 4 ? columns : vocab;
+  if (vocab < 4) HELD(1, 1, 4, 4);
+  if (narrow <= 16) HELD(4, 1, 4, 4);
+  if (narrow <= 32) HELD(4, 1, 8, 4);
+  if (narrow <= 64) HELD(4, 1, 16, 2 * V);
+  if (narrow <= 128) HELD(4, 1, 32, 2 * V);
+  if (narrow <= 256) HELD(4, 1, 64, 2 * V);
+  if (narrow <= 512) HELD(4, 2, 64, V);
+  if (narrow <= 1024) HELD(4, 4, 64, V / 2);
+  if (narrow <= 2048) HELD(4, 8, 64, 1);
+  if (p->dlogits) {
+    // Several rows a CU hide each other's reductions, so a row takes as few threads as its registers allow.  Measured on an
+    // MI355X, bf16, gradient read and write of 200 million logits: 16384 columns in 256 threads 161 us, in 1024 226;
+    // 32768 in 512 161, 256 169, 1024 187; 49999 in 512 200, 256 241, 1024 202.
+    if (columns <= 256 * W * 4) HELD(W, 4, 256, 1);
+    if (columns <= 256 * W * 8) HELD(W, 8, 256, 1);
+    if (columns <= 512 * W * 8) HELD(W, 8, 512, 1);
+    if (columns <= 512 * W * 12) HELD(W, 12, 512, 1);
+    if (columns <= 512 * W * 16) HELD(W, 16, 512, 1);
+    if (columns <= 1024 * W * 16) HELD(W, 16, 1024, 1);
+  }
+#undef HELD
+  *n_parts = rows;
+  if (p->dlogits)
+    hipLaunchKernelGGL((policy_swept_kernel<T, W, true>), dim3((unsigned)rows), dim3(SWEEP), 0, st, P, (const T*)p->logits, (T*)p->dlogits, parts);
+  else
+    hipLaunchKernelGGL((policy_swept_kernel<T, W, false>), dim3((unsigned)rows), dim3(SWEEP), 0, st, P, (const T*)p->logits, (T*)nullptr, parts);
 }
 
 }  // namespace
@@ -163,7 +550,8 @@ extern "C" {
 int rlgan_policy_loss_workspace(int64_t rows, int vocab, int type, int64_t* bytes) {
   if (!bytes || rows <= 0 || vocab <= 0) return RLGAN_E_ARG;
   if (type < TYPE_F32 || type > TYPE_F16) return RLGAN_E_KIND;
-  *bytes = rows * 8;
+  const Cuts cut = cuts_of(rows, vocab, type);
+  *bytes = rows * 8 + (cut.count > 1 ? rows * cut.count * (int64_t)sizeof(Stats) + rows * 4 : 0);
   return 0;
 }
 
@@ -176,13 +564,11 @@ int rlgan_policy_loss(const rlgan_policy_t* p, void* workspace, void* stream) {
   if (!(p->temperature > 0)) return RLGAN_E_ARG;
   Policy P{p->rows, p->vocab, p->ld, p->ld_legal, p->ld_d, p->actions, p->action_bytes == 8, p->old_logp, p->advantages, p->weights, p->ref_logp,
            p->legal, (float)(1.44269504088896340736 / p->temperature), 1.0 / p->temperature, p->clip_low, p->clip_high, p->kl_coef,
-           p->entropy_coef, 1.0 / (double)p->rows, p->logp, p->entropy, p->kl, (double*)workspace};
+           p->entropy_coef, 1.0 / (double)p->rows, p->logp, p->entropy, p->kl};
   hipStream_t st = (hipStream_t)stream;
-  RLGAN_BY_TYPE(p->type, T, {
-    if (p->dlogits) hipLaunchKernelGGL((policy_rows_kernel<T, true>), dim3((unsigned)p->rows), dim3(256), 0, st, P, (const T*)p->logits, (T*)p->dlogits);
-    else hipLaunchKernelGGL((policy_rows_kernel<T, false>), dim3((unsigned)p->rows), dim3(256), 0, st, P, (const T*)p->logits, (T*)nullptr);
-  });
-  hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(1024), 0, st, (const double*)workspace, p->rows, p->loss);
+  int64_t n_parts = 0;
+  RLGAN_BY_TYPE(p->type, T, launch_rows<T>(P, p, workspace, &n_parts, st));
+  hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(1024), 0, st, (const double*)workspace, n_parts, p->loss);
   return (int)hipGetLastError();
 }
 
