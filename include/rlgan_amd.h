@@ -668,6 +668,10 @@ typedef struct {
 int rlgan_gated_scan_workspace(int batch, int length, int width, int type, int backward, int64_t* bytes);
 /* h [batch][length][width] and the state behind each sequence's last step */
 int rlgan_gated_scan_forward(const rlgan_scan_t* s, rlgan_seq_t h, float* state_out, void* workspace, void* stream);
+/* One step of acting: z, x [batch] rows of `width` channels (row strides in elements), the state advanced in place, h dense
+ * [batch][width]; starts: one byte a row at starts[b * starts_batch], or NULL. */
+int rlgan_gated_step(int type, int batch, int width, const void* z, int64_t z_batch, const void* x, int64_t x_batch, float* state,
+                     const uint8_t* starts, int64_t starts_batch, void* h, void* stream);
 /* Gradient: h of the forward pass, dh the gradient of h, dstate of the final state (NULL: zeros) -> dz, dx, and dstate_in of the
  * state handed in:  g_t = dh_t + f_{t+1} keep_{t+1} g_{t+1},  dx = (1 - f) g,  dz = g (p - x) f (1 - f). */
 int rlgan_gated_scan_backward(const rlgan_scan_t* s, rlgan_seq_t h, rlgan_seq_t dh, const float* dstate, rlgan_seq_t dz, rlgan_seq_t dx,

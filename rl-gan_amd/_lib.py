@@ -269,6 +269,7 @@ PROTOTYPES = {
     "rlgan_gated_scan_workspace": [_i, _i, _i, _i, _i, C.POINTER(C.c_int64)],
     "rlgan_gated_scan_forward": [C.POINTER(Scan), SeqRef, _vp, _vp, _vp],
     "rlgan_gated_scan_backward": [C.POINTER(Scan), SeqRef, SeqRef, _vp, SeqRef, SeqRef, _vp, _vp, _vp],
+    "rlgan_gated_step": [_i, _i, _i, _vp, C.c_int64, _vp, C.c_int64, _vp, _vp, C.c_int64, _vp, _vp],
     "rlgan_policy_loss_workspace": [C.c_int64, _i, _i, C.POINTER(C.c_int64)],
     "rlgan_policy_loss": [C.POINTER(Policy), _vp, _vp],
     "rlgan_adamw_step": [C.POINTER(AdamWState), _vp, _vp, _vp, _vp, _vp],

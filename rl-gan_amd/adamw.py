@@ -3,6 +3,7 @@ tensors (`DenseLayer.canon`, `GatedUnit.gates.canon`, a caller's own), beside th
 (`rlgan_apply`, DDPG.py:69,145, Curious_GAN.py:37-42)."""
 from __future__ import annotations
 
+import array
 import ctypes as C
 from typing import List, Optional, Sequence, Tuple
 
@@ -47,7 +48,7 @@ class AdamW:
         self._chunk_begin = np.ascontiguousarray(np.concatenate([[0], np.cumsum(n_chunks)]).astype(np.int64))
         which = np.repeat(np.arange(len(counts)), n_chunks)
         table = np.stack([which, np.arange(len(which)) - self._chunk_begin[which]], 1).astype(np.int32)
-        self._ptrs = [p.data_ptr() for p in self.params]
+        self._ptrs, self._shapes = [p.data_ptr() for p in self.params], [p.shape for p in self.params]
         records = (AdamWTensor * len(counts))(*[AdamWTensor(q, int(n), int(o), TYPES[p.dtype], 0)
                                                 for q, n, o, p in zip(self._ptrs, counts, self.offsets, self.params)])
         up = lambda a: torch.from_numpy(a).to(dev)
@@ -78,15 +79,13 @@ class AdamW:
         device scalar that multiplies the gradients (1 / loss scale, what clipping by a norm left).  skip: bool device scalar;
         where it is True nothing changes (gradients of a scaled loss that overflowed)."""
         need(len(grads) == len(self.params), f"{len(grads)} gradients for {len(self.params)} parameters")
-        n, dev = len(grads), self.device
-        pointers, types = (C.c_void_p * n)(), (C.c_uint8 * n)()
-        for i, (p, q, g) in enumerate(zip(self.params, self._ptrs, grads)):
-            code = TYPES.get(g.dtype)
-            if code is None or g.device != dev or g.shape != p.shape or not g.is_contiguous():
-                raise ValueError(f"grads[{i}]: a contiguous float32, bfloat16 or float16 tensor of shape {tuple(p.shape)} on {dev} is wanted")
-            if p.data_ptr() != q:
-                raise ValueError(f"params[{i}] has moved in memory since the optimizer was made")
-            pointers[i], types[i] = g.data_ptr(), code
+        dev = self.device
+        # whole lists are compared first: a call with nothing wrong stays out of the loop that says what is
+        if ([g.shape for g in grads] != self._shapes or [p.data_ptr() for p in self.params] != self._ptrs or
+                not all([g.is_contiguous() and g.dtype in TYPES for g in grads]) or {g.get_device() for g in grads} != {dev.index}):
+            self._refuse(grads)
+        pointers = array.array("Q", [g.data_ptr() for g in grads])
+        types = bytes([TYPES[g.dtype] for g in grads])
         p_scale = p_skip = None
         if grad_scale is not None:
             on_device(grad_scale, dev, "grad_scale")
@@ -97,7 +96,15 @@ class AdamW:
             need(skip.dtype in (torch.bool, torch.uint8) and skip.numel() == 1, "skip: one bool on the device")
             p_skip = skip.data_ptr()
         with guard(dev):
-            check(lib.rlgan_adamw_step(C.byref(self._state), pointers, types, p_scale, p_skip, stream_of(dev)), "rlgan_adamw_step")
+            check(lib.rlgan_adamw_step(C.byref(self._state), pointers.buffer_info()[0], types, p_scale, p_skip, stream_of(dev)), "rlgan_adamw_step")
+
+    def _refuse(self, grads) -> None:
+        for i, (p, q, g) in enumerate(zip(self.params, self._ptrs, grads)):
+            if g.dtype not in TYPES or g.device != self.device or g.shape != p.shape or not g.is_contiguous():
+                raise ValueError(f"grads[{i}]: a contiguous float32, bfloat16 or float16 tensor of shape {tuple(p.shape)} on {self.device} is wanted")
+            if p.data_ptr() != q:
+                raise ValueError(f"params[{i}] has moved in memory since the optimizer was made")
+        raise ValueError("parameters have changed since the optimizer was made")
 
     # ---- state -------------------------------------------------------------------------------------
     def moments(self) -> Tuple[torch.Tensor, torch.Tensor]:

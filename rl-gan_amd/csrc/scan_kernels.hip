@@ -505,6 +505,13 @@ int rlgan_gated_scan_forward(const rlgan_scan_t* s, rlgan_seq_t h, float* state_
   return (int)hipGetLastError();
 }
 
+int rlgan_gated_step(int type, int batch, int width, const void* z, int64_t z_batch, const void* x, int64_t x_batch, float* state,
+                     const uint8_t* starts, int64_t starts_batch, void* h, void* stream) {
+  if (!state) return RLGAN_E_ARG;
+  const rlgan_scan_t s{batch, 1, width, type, {(void*)z, z_batch, 0}, {(void*)x, x_batch, 0}, state, starts, starts_batch, 0, nullptr};
+  return rlgan_gated_scan_forward(&s, {h, width, 0}, state, nullptr, stream);
+}
+
 int rlgan_gated_scan_backward(const rlgan_scan_t* s, rlgan_seq_t h, rlgan_seq_t dh, const float* dstate, rlgan_seq_t dz, rlgan_seq_t dx,
                               float* dstate_in, void* workspace, void* stream) {
   if (int e = check_scan(s)) return e;

@@ -9,7 +9,7 @@ from typing import NamedTuple, Optional, Tuple, Union
 import torch
 
 from ._lib import Policy, check, lib
-from .tensors import apart, first_device, guard, need, on_device, own_elements, stream_of, type_code, vector, workspace
+from .tensors import apart, first_device, guard, need, on_device, own_elements, stream_of, type_code, vector
 
 
 class PolicyLoss(NamedTuple):
@@ -79,16 +79,20 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logp: torch.Ten
         none = torch.zeros(0, dtype=torch.float32, device=dev)
         return PolicyLoss(torch.zeros((), dtype=torch.float32, device=dev), none, none.clone(), none.clone(), d)
     with guard(dev):
-        stats = torch.empty((4, rows), dtype=torch.float32, device=dev)
         size = C.c_int64()
         check(lib.rlgan_policy_loss_workspace(rows, vocab, code, C.byref(size)), "rlgan_policy_loss_workspace")
-        ws = workspace(size.value, dev)
-        base = stats.data_ptr()
+        # the workspace (8-byte sums in front), then the three rows of results: one allocation of this call alone
+        words = (size.value + 3) // 4
+        room = torch.empty(words + 3 * rows, dtype=torch.float32, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        base = room.data_ptr()
+        out_at = base + 4 * words
         args = Policy(rows, vocab, code, logits.data_ptr(), ld, actions.data_ptr(), actions.element_size(), p_old, p_adv, p_w, p_ref, p_legal,
-                      ld_legal, low, high, kl_coef, entropy_coef, temperature, base, base + 4 * rows, base + 8 * rows, base + 12 * rows,
+                      ld_legal, low, high, kl_coef, entropy_coef, temperature, loss.data_ptr(), out_at, out_at + 4 * rows, out_at + 8 * rows,
                       None if d is None else d.data_ptr(), 0 if d is None else _row_stride(d, vocab))
-        check(lib.rlgan_policy_loss(C.byref(args), ws.data_ptr(), stream_of(dev)), "rlgan_policy_loss")
-    return PolicyLoss(stats[0, 0], stats[1], stats[2], stats[3], d)
+        check(lib.rlgan_policy_loss(C.byref(args), base, stream_of(dev)), "rlgan_policy_loss")
+    _, logp, entropy, kl = room.split([words, rows, rows, rows])
+    return PolicyLoss(loss, logp, entropy, kl, d)
 
 
 def _row_stride(t: torch.Tensor, vocab: int) -> int:

@@ -17,7 +17,7 @@ import torch
 
 from ._lib import Scan, SeqRef, check, lib
 from .conv import DenseLayer
-from .tensors import apart, first_device, guard, need, on_device, stream_of, type_code, vector, workspace
+from .tensors import apart, byte_range, first_device, guard, need, on_device, stream_of, type_code, vector, workspace
 
 
 def _seq(t: torch.Tensor, shape, dtype, dev, name: str) -> SeqRef:
@@ -122,16 +122,34 @@ def _halves_apart(a: torch.Tensor, b: torch.Tensor) -> None:
 def gated_step(z: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *, starts: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One step of acting: z and x [batch, width], state [batch, width] float32, advanced in place; returns h in z's type.
     starts: bool [batch], True where the state is not to be used because an episode begins."""
-    need(isinstance(z, torch.Tensor) and isinstance(x, torch.Tensor) and z.dim() == 2 and x.dim() == 2, "z and x are [batch, width]")
-    need(starts is None or starts.dim() == 1, "starts: [batch]")
+    dev = first_device(z, "z")
+    code = type_code(z, "z")
+    shape = z.shape
+    need(len(shape) == 2, "z and x are [batch, width]")
+    on_device(x, dev, "x")
+    if x.dtype != z.dtype or x.shape != shape:
+        raise ValueError(f"x: {z.dtype} of shape {tuple(shape)} is wanted, got {x.dtype} {tuple(x.shape)}")
+    b, d = shape
+    (zb, zc), (xb, xc) = z.stride(), x.stride()
+    need(d <= 1 or zc == xc == 1, "z and x: channels have to lie next to each other")
+    need(b * d <= 1 << 31, "at most 2^31 units")
     need(state is not None, "state: a float32 tensor [batch, width] to advance")
-    s, dev = _scan(z[:, None], x[:, None], state, None if starts is None else starts[:, None], None)
-    apart(state, (z, x, starts), "state")
-    h = torch.empty(z.shape, dtype=z.dtype, device=dev)
-    if z.numel():
-        with guard(dev):
-            check(lib.rlgan_gated_scan_forward(C.byref(s), SeqRef(h.data_ptr(), s.width, s.width), state.data_ptr(), None, stream_of(dev)),
-                  "rlgan_gated_scan_forward")
+    p_state = vector(state, shape, dev, "state")
+    p_starts = starts_b = None
+    if starts is not None:
+        on_device(starts, dev, "starts")
+        need(starts.dtype in (torch.bool, torch.uint8) and starts.shape == shape[:1], "starts: bool or uint8 of shape [batch]")
+        p_starts, starts_b = starts.data_ptr(), starts.stride(0)
+    h = torch.empty(shape, dtype=z.dtype, device=dev)
+    if h.numel() == 0:
+        return h
+    lo, hi = p_state, p_state + 4 * b * d
+    for t in (z, x) if starts is None else (z, x, starts):
+        first, end = byte_range(t)
+        need(end <= lo or hi <= first, "state shares memory with another tensor of the call")
+    with guard(dev):
+        check(lib.rlgan_gated_step(code, b, d, z.data_ptr(), zb, x.data_ptr(), xb, p_state, p_starts, starts_b or 0, h.data_ptr(), stream_of(dev)),
+              "rlgan_gated_step")
     return h
 
 

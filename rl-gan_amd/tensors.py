@@ -48,9 +48,15 @@ def vector(t: Optional[torch.Tensor], shape, dev: torch.device, name: str, dtype
 
 def byte_range(t: torch.Tensor):
     """First byte of a tensor and the one behind its last."""
+    at = t.data_ptr()
+    if t.is_contiguous():
+        return at, at + t.numel() * t.element_size()
     if t.numel() == 0:
-        return t.data_ptr(), t.data_ptr()
-    return t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+        return at, at
+    last = 1
+    for n, s in zip(t.shape, t.stride()):
+        last += (n - 1) * s
+    return at, at + last * t.element_size()
 
 
 def apart(out: torch.Tensor, others, name: str) -> None:
@@ -77,11 +83,16 @@ def own_elements(t: torch.Tensor, name: str) -> None:
 
 def guard(dev: torch.device):
     """Makes `dev` the current device for the launches of a call."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+_HERE = contextlib.nullcontext()
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)     # the handle without a Stream object around it
 
 
 def stream_of(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    """The device's current stream."""
+    return _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
 def workspace(size: int, dev: torch.device) -> Optional[torch.Tensor]:

@@ -52,6 +52,14 @@ def test_scan_refusals():
     assert lib.rlgan_gated_scan_workspace(2, 3, 4, 7, 0, C.byref(n)) == KIND
 
 
+def test_step_refusals():
+    ok = [0, 2, 4, 64, 4, 64, 4, 64, None, 0, 64, None]
+    for at, value, want in ((0, 3, KIND), (1, 0, ARG), (2, -1, ARG), (3, None, ARG), (5, None, ARG), (7, None, ARG), (10, None, ARG)):
+        args = list(ok)
+        args[at] = value
+        assert lib.rlgan_gated_step(*args) == want, at
+
+
 def test_scan_workspace_is_wanted():
     """A long sequence of few units is cut, and its call wants the workspace that the size function names."""
     n = C.c_int64()
