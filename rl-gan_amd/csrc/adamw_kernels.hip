@@ -31,16 +31,32 @@ __global__ void adamw_begin_kernel(int32_t* step, const float* lr, double beta1,
   out->skip = no;
 }
 
-template <typename T> __device__ __forceinline__ void load4(const void* base, int64_t i, int64_t n, float v[4]) {
-  const T* p = (const T*)base + i;
-  if (i + 4 <= n) {
-    Vec<T, 4> u;
-    u.load(p);
+// 4 elements from the i-th on as they lie in memory, and as floats: apart, so that a workgroup's loads are all in flight before the
+// first conversion waits for one (the type is known at run time only).  Behind the n-th: zeros.
+struct Raw4 { uint32_t w[4]; };
+template <typename T> __device__ __forceinline__ void load_raw(const T* p, int64_t i, int64_t n, Raw4& r) {
+  if (i + 4 <= n) __builtin_memcpy(r.w, p + i, 4 * sizeof(T));
+  else {
+    T v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = u.get(k);
+    for (int k = 0; k < 4; ++k) v[k] = i + k < n ? p[i + k] : (T)0.f;
+    __builtin_memcpy(r.w, v, sizeof(v));
+  }
+}
+__device__ __forceinline__ void load_raw(int type, const void* p, int64_t i, int64_t n, Raw4& r) {
+  if (type == TYPE_F32) load_raw<uint32_t>((const uint32_t*)p, i, n, r);
+  else load_raw<uint16_t>((const uint16_t*)p, i, n, r);
+}
+__device__ __forceinline__ void as_floats(int type, const Raw4& r, float v[4]) {
+  if (type == TYPE_F32) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(r.w[k]);
+  } else if (type == TYPE_BF16) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(k & 1 ? r.w[k / 2] & 0xFFFF0000u : r.w[k / 2] << 16);
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = i + k < n ? (float)p[k] : 0.f;
+    for (int k = 0; k < 4; ++k) v[k] = (float)__builtin_bit_cast(f16_t, (uint16_t)(r.w[k / 2] >> (16 * (k & 1))));
   }
 }
 template <typename T> __device__ __forceinline__ void store4(void* base, int64_t i, int64_t n, const float v[4]) {
@@ -55,9 +71,6 @@ template <typename T> __device__ __forceinline__ void store4(void* base, int64_t
     for (int k = 0; k < 4; ++k) if (i + k < n) p[k] = (T)v[k];
   }
 }
-__device__ __forceinline__ void load4(int type, const void* base, int64_t i, int64_t n, float v[4]) {
-  RLGAN_BY_TYPE(type, T, load4<T>(base, i, n, v));
-}
 
 // 8-bit floats: MAN mantissa bits, COUNT magnitudes
 template <int MAN, int COUNT> struct Small {
@@ -65,10 +78,15 @@ template <int MAN, int COUNT> struct Small {
   // a magnitude rounded to MAN bits behind the leading one (ties to even), in units of that bit with a 32-bit float's exponent;
   // 0 under the normal range, at least 255 << MAN for what no float holds
   static __device__ __forceinline__ int rounded(double v) {
-    const uint64_t b = (uint64_t)__double_as_longlong(v) & 0x7FFFFFFFFFFFFFFFull;
-    const uint64_t r = (b + ((1ull << (51 - MAN)) - 1) + ((b >> (52 - MAN)) & 1)) >> (52 - MAN);
-    const int64_t u = (int64_t)r - ((int64_t)896 << MAN);
-    return u < (1 << MAN) ? 0 : u > (255 << MAN) ? 255 << MAN : (int)u;
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    const uint32_t h = ((uint32_t)(b >> 32) & 0x7FFFFFFFu) | ((uint32_t)b != 0);     // what lies below counts only as "more than"
+    const int u = (int)((h + ((1u << (19 - MAN)) - 1) + ((h >> (20 - MAN)) & 1)) >> (20 - MAN)) - (896 << MAN);
+    return u < (1 << MAN) ? 0 : min(u, 255 << MAN);
+  }
+  // the same of a normal float that is known to `slack` units of its last place; -1 where that does not decide
+  static __device__ __forceinline__ int rounded(float v, int slack) {
+    const int b = __float_as_int(v), half = 1 << (22 - MAN), rest = (b & (2 * half - 1)) - half;
+    return abs(rest) <= slack ? -1 : (b + half) >> (23 - MAN);
   }
   static __device__ __forceinline__ int code(int r, int exponent, bool keep) {
     if (r == 0) return 0;
@@ -101,11 +119,11 @@ __device__ __forceinline__ void decode4(uint32_t cm, int em, uint32_t cr, int er
   }
 }
 
-__device__ __forceinline__ void encode4(const double m[4], const double root[4], uint32_t& cm, int& em, uint32_t& cr, int& er) {
-  int rm[4], rr[4], hm = 0, hr = 0;
+__device__ __forceinline__ void encode4(const double m[4], const int rr[4], uint32_t& cm, int& em, uint32_t& cr, int& er) {
+  int rm[4], hm = 0, hr = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    rm[k] = First::rounded(m[k]); rr[k] = Root::rounded(root[k]);
+    rm[k] = First::rounded(m[k]);
     hm = max(hm, rm[k]); hr = max(hr, rr[k]);
   }
   em = block_max(hm) >> 3; er = block_max(hr) >> 4;
@@ -130,16 +148,39 @@ __global__ __launch_bounds__(256) void adamw_kernel(const rlgan_adamw_tensor_t* 
   const int gt = grads.type[ti - tensor0];
   const float gs = grad_scale ? *grad_scale : 1.f;
   const int64_t begin = (int64_t)ci * CHUNK, padded = (T.count + BLOCK - 1) / BLOCK * BLOCK;
-  for (int64_t i = begin + 4 * threadIdx.x; i < begin + CHUNK && i < padded; i += 1024) {
-    float p[4], g[4], m[4], root[4];
-    load4(T.type, T.param, i, T.count, p);
-    load4(gt, gp, i, T.count, g);
+  constexpr int TURNS = CHUNK / 1024;
+  Raw4 rp[TURNS], rg[TURNS];
+  float4 rm[TURNS], rv[TURNS];
+  uint32_t cm[TURNS], cr[TURNS];
+  int em[TURNS], er[TURNS];
+#pragma unroll
+  for (int u = 0; u < TURNS; ++u) {
+    const int64_t i = begin + 1024 * u + 4 * threadIdx.x;
+    if (i >= padded) continue;                                   // the 16 lanes of a block go together
     const int64_t at = T.offset + i;
+    load_raw(T.type, T.param, i, T.count, rp[u]);
+    load_raw(gt, gp, i, T.count, rg[u]);
     if constexpr (BITS == 32) {
-      float v[4];
-      float* mp = (float*)first_ + at; float* vp = (float*)second_ + at;
-      __builtin_memcpy(m, __builtin_assume_aligned(mp, 16), 16);
-      __builtin_memcpy(v, __builtin_assume_aligned(vp, 16), 16);
+      rm[u] = ((const float4*)first_)[at / 4];
+      rv[u] = ((const float4*)second_)[at / 4];
+    } else {
+      cm[u] = ((const uint32_t*)first_)[at / 4];
+      cr[u] = ((const uint32_t*)second_)[at / 4];
+      em[u] = first_e[at / BLOCK];
+      er[u] = second_e[at / BLOCK];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < TURNS; ++u) {
+    const int64_t i = begin + 1024 * u + 4 * threadIdx.x;
+    if (i >= padded) continue;
+    const int64_t at = T.offset + i;
+    float p[4], g[4], m[4], root[4];
+    as_floats(T.type, rp[u], p);
+    as_floats(gt, rg[u], g);
+    if constexpr (BITS == 32) {
+      m[0] = rm[u].x; m[1] = rm[u].y; m[2] = rm[u].z; m[3] = rm[u].w;
+      float v[4] = {rv[u].x, rv[u].y, rv[u].z, rv[u].w};
       const float b1 = (float)beta1, c1 = (float)(1.0 - beta1), b2 = (float)beta2, c2 = (float)(1.0 - beta2);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -148,31 +189,49 @@ __global__ __launch_bounds__(256) void adamw_kernel(const rlgan_adamw_tensor_t* 
         v[k] = v[k] * b2 + gk * c2 * gk;
         root[k] = sqrtf(v[k]);
       }
-      __builtin_memcpy(__builtin_assume_aligned(mp, 16), m, 16);
-      __builtin_memcpy(__builtin_assume_aligned(vp, 16), v, 16);
+      ((float4*)first_)[at / 4] = make_float4(m[0], m[1], m[2], m[3]);
+      ((float4*)second_)[at / 4] = make_float4(v[0], v[1], v[2], v[3]);
     } else {
-      // 64 bits up to the codes, without contraction: b1 m + (1 - b1) g of values with so few bits lands on the border between
-      // two codes often enough (15 * 0.9 = 13.5), and 32 bits would decide by their own rounding there
+      // Codes are decided by 64-bit arithmetic, without contraction: b1 m + (1 - b1) g of values with so few bits lands on the border
+      // between two codes often enough (15 * 0.9 = 13.5), and 32 bits would decide by their own rounding there.  The root's are
+      // decided in 32 bits where the nearest border is further than those can err (6 roundings of the sum, halved by the root, and that of
+      // the root instruction: 5 units of the last place; 16 are allowed for), and in 64 elsewhere: some 1 in 16000 elements, and where
+      // v is not between 1e-30 and 1e30.
 #pragma clang fp contract(off)
-      uint32_t* mp = (uint32_t*)first_ + at / 4; uint32_t* rp = (uint32_t*)second_ + at / 4;
-      uint8_t* me = first_e + at / BLOCK; uint8_t* re = second_e + at / BLOCK;
-      decode4(*mp, *me, *rp, *re, m, root);
-      double dm[4], dr[4];
+      decode4(cm[u], em[u], cr[u], er[u], m, root);
+      double dm[4];
+      int rr[4];
+      const float b2 = (float)beta2, c2 = (float)(1.0 - beta2);
+      bool unsure = false;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const double gk = (double)g[k] * (double)gs, r = root[k];
-        dm[k] = (double)m[k] * beta1 + gk * (1.0 - beta1);
-        dr[k] = sqrt(r * r * beta2 + gk * (1.0 - beta2) * gk);
-        m[k] = (float)dm[k]; root[k] = (float)dr[k];
+        dm[k] = (double)m[k] * beta1 + (double)g[k] * (double)gs * (1.0 - beta1);
+        m[k] = (float)dm[k];
+        const float gk = g[k] * gs, v = root[k] * root[k] * b2 + gk * c2 * gk, s = __builtin_amdgcn_sqrtf(v);
+        rr[k] = v == 0.f ? 0 : Root::rounded(s, 16);
+        const bool known = rr[k] >= 0 && (v == 0.f ? gk == 0.f && root[k] == 0.f : v > 1e-30f && v < 1e30f);
+        rr[k] = known ? rr[k] : -1;
+        unsure = unsure || !known;
+        if (known) root[k] = s;
       }
-      uint32_t cm, cr;
-      int em, er;
-      encode4(dm, dr, cm, em, cr, er);
-      *mp = cm; *rp = cr;
-      if ((threadIdx.x & 15) == 0) { *me = (uint8_t)em; *re = (uint8_t)er; }
+      if (unsure) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (rr[k] >= 0) continue;
+          const double gk = (double)g[k] * (double)gs, r = root[k], s = sqrt(r * r * beta2 + gk * (1.0 - beta2) * gk);
+          rr[k] = Root::rounded(s);
+          root[k] = (float)s;
+        }
+      }
+      uint32_t nm, nr;
+      int fm, fr;
+      encode4(dm, rr, nm, fm, nr, fr);
+      ((uint32_t*)first_)[at / 4] = nm;
+      ((uint32_t*)second_)[at / 4] = nr;
+      if ((threadIdx.x & 15) == 0) { first_e[at / BLOCK] = (uint8_t)fm; second_e[at / BLOCK] = (uint8_t)fr; }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) p[k] = p[k] * sc.keep - sc.lr_t * (m[k] / (root[k] * sc.root_t + eps));
+    for (int k = 0; k < 4; ++k) p[k] = p[k] * sc.keep - sc.lr_t * m[k] * __builtin_amdgcn_rcpf(root[k] * sc.root_t + eps);
     RLGAN_BY_TYPE(T.type, E, store4<E>(T.param, i, T.count, p));
   }
 }
@@ -193,9 +252,10 @@ __global__ __launch_bounds__(256) void adamw_encode_kernel(const float4* m_in, c
   if (i >= n4) return;                              // n4 is a multiple of 16: whole blocks leave together
   const float4 a = m_in[i], b = v_in[i];
   const double m[4] = {a.x, a.y, a.z, a.w}, r[4] = {sqrt((double)b.x), sqrt((double)b.y), sqrt((double)b.z), sqrt((double)b.w)};
+  const int rr[4] = {Root::rounded(r[0]), Root::rounded(r[1]), Root::rounded(r[2]), Root::rounded(r[3])};
   uint32_t cm, cr;
   int em, er;
-  encode4(m, r, cm, em, cr, er);
+  encode4(m, rr, cm, em, cr, er);
   first[i] = cm; second[i] = cr;
   if ((threadIdx.x & 15) == 0) { first_e[i / 16] = (uint8_t)em; second_e[i / 16] = (uint8_t)er; }
 }
