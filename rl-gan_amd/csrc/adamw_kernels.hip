@@ -34,8 +34,8 @@ __global__ void adamw_begin_kernel(int32_t* step, const float* lr, double beta1,
 // 4 elements from the i-th on as they lie in memory, and as floats: apart, so that a workgroup's loads are all in flight before the
 // first conversion waits for one (the type is known at run time only).  Behind the n-th: zeros.
 struct Raw4 { uint32_t w[4]; };
-template <typename T> __device__ __forceinline__ void load_raw(const T* p, int64_t i, int64_t n, Raw4& r) {
-  if (i + 4 <= n) __builtin_memcpy(r.w, p + i, 4 * sizeof(T));
+template <bool FULL, typename T> __device__ __forceinline__ void load_raw(const T* p, int i, int n, Raw4& r) {
+  if (FULL || i + 4 <= n) __builtin_memcpy(r.w, p + i, 4 * sizeof(T));
   else {
     T v[4];
 #pragma unroll
@@ -43,9 +43,9 @@ template <typename T> __device__ __forceinline__ void load_raw(const T* p, int64
     __builtin_memcpy(r.w, v, sizeof(v));
   }
 }
-__device__ __forceinline__ void load_raw(int type, const void* p, int64_t i, int64_t n, Raw4& r) {
-  if (type == TYPE_F32) load_raw<uint32_t>((const uint32_t*)p, i, n, r);
-  else load_raw<uint16_t>((const uint16_t*)p, i, n, r);
+template <bool FULL> __device__ __forceinline__ void load_raw(int type, const void* p, int64_t begin, int i, int n, Raw4& r) {
+  if (type == TYPE_F32) load_raw<FULL>((const uint32_t*)p + begin, i, n, r);
+  else load_raw<FULL>((const uint16_t*)p + begin, i, n, r);
 }
 __device__ __forceinline__ void as_floats(int type, const Raw4& r, float v[4]) {
   if (type == TYPE_F32) {
@@ -59,9 +59,9 @@ __device__ __forceinline__ void as_floats(int type, const Raw4& r, float v[4]) {
     for (int k = 0; k < 4; ++k) v[k] = (float)__builtin_bit_cast(f16_t, (uint16_t)(r.w[k / 2] >> (16 * (k & 1))));
   }
 }
-template <typename T> __device__ __forceinline__ void store4(void* base, int64_t i, int64_t n, const float v[4]) {
-  T* p = (T*)base + i;
-  if (i + 4 <= n) {
+template <bool FULL, typename T> __device__ __forceinline__ void store4(void* base, int64_t begin, int i, int n, const float v[4]) {
+  T* p = (T*)base + begin + i;
+  if (FULL || i + 4 <= n) {
     Vec<T, 4> u;
 #pragma unroll
     for (int k = 0; k < 4; ++k) u.set(k, v[k]);
@@ -89,14 +89,12 @@ template <int MAN, int COUNT> struct Small {
     return abs(rest) <= slack ? -1 : (b + half) >> (23 - MAN);
   }
   static __device__ __forceinline__ int code(int r, int exponent, bool keep) {
-    if (r == 0) return 0;
-    const int c = r - ((exponent << MAN) | ONES) + COUNT;
-    return c < 1 ? (keep ? 1 : 0) : c;
+    const int c = max(r - ((exponent << MAN) | ONES) + COUNT, keep ? 1 : 0);
+    return r == 0 ? 0 : c;
   }
   static __device__ __forceinline__ float value(int c, int exponent) {
-    if (exponent == 255) return __builtin_nanf("");
-    const int r = ((exponent << MAN) | ONES) - COUNT + c;
-    return c > 0 && r > ONES ? __int_as_float(r << (23 - MAN)) : 0.f;
+    const int r = ((exponent << MAN) | ONES) - COUNT + c, bits = (c > 0) & (r > ONES) ? r << (23 - MAN) : 0;
+    return __int_as_float(exponent == 255 ? 0x7FC00000 : bits);
   }
 };
 typedef Small<3, 127> First;
@@ -113,8 +111,7 @@ __device__ __forceinline__ void decode4(uint32_t cm, int em, uint32_t cr, int er
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int c = (cm >> (8 * k)) & 255;
-    const float v = First::value(c & 127, em);
-    m[k] = c > 127 ? -v : v;
+    m[k] = __int_as_float(__float_as_int(First::value(c & 127, em)) | (c & 128) << 24);
     root[k] = Root::value((cr >> (8 * k)) & 255, er);
   }
 }
@@ -131,57 +128,51 @@ __device__ __forceinline__ void encode4(const double m[4], const int rr[4], uint
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int c = First::code(rm[k], em, false);
-    cm |= (uint32_t)(c | (c && m[k] < 0 ? 128 : 0)) << (8 * k);
+    cm |= (uint32_t)(c | ((c > 0) & (m[k] < 0) ? 128 : 0)) << (8 * k);
     cr |= (uint32_t)Root::code(rr[k], er, true) << (8 * k);
   }
 }
 
-template <int BITS>
-__global__ __launch_bounds__(256) void adamw_kernel(const rlgan_adamw_tensor_t* tensors, const int32_t* chunks, int64_t chunk0, int tensor0,
-                                                    Grads grads, void* first_, void* second_, uint8_t* first_e, uint8_t* second_e,
-                                                    double beta1, double beta2, float eps, const float* grad_scale, const Scalars* scalars) {
-  const Scalars sc = *scalars;
-  if (sc.skip) return;
-  const int ti = chunks[2 * (chunk0 + blockIdx.x)], ci = chunks[2 * (chunk0 + blockIdx.x) + 1];
-  const rlgan_adamw_tensor_t T = tensors[ti];
-  const void* gp = grads.p[ti - tensor0];
-  const int gt = grads.type[ti - tensor0];
-  const float gs = grad_scale ? *grad_scale : 1.f;
-  const int64_t begin = (int64_t)ci * CHUNK, padded = (T.count + BLOCK - 1) / BLOCK * BLOCK;
+struct Rates { double beta1, beta2; float eps, scale; };
+
+// the chunk of n elements (FULL: all of CHUNK) that begins at p's and g's `begin`; the state's pointers are the chunk's
+template <int BITS, bool FULL>
+__device__ __forceinline__ void adamw_chunk(int pt, void* pp, int gt, const void* gp, int64_t begin, int n, void* first_, void* second_,
+                                            uint8_t* first_e, uint8_t* second_e, const Rates& rate, const Scalars& sc) {
+  const int padded = (n + BLOCK - 1) / BLOCK * BLOCK;
   constexpr int TURNS = CHUNK / 1024;
+  const float gs = rate.scale;
   Raw4 rp[TURNS], rg[TURNS];
   float4 rm[TURNS], rv[TURNS];
   uint32_t cm[TURNS], cr[TURNS];
   int em[TURNS], er[TURNS];
 #pragma unroll
   for (int u = 0; u < TURNS; ++u) {
-    const int64_t i = begin + 1024 * u + 4 * threadIdx.x;
-    if (i >= padded) continue;                                   // the 16 lanes of a block go together
-    const int64_t at = T.offset + i;
-    load_raw(T.type, T.param, i, T.count, rp[u]);
-    load_raw(gt, gp, i, T.count, rg[u]);
+    const int i = 1024 * u + 4 * threadIdx.x;
+    if (!FULL && i >= padded) continue;                          // the 16 lanes of a block go together
+    load_raw<FULL>(pt, pp, begin, i, n, rp[u]);
+    load_raw<FULL>(gt, gp, begin, i, n, rg[u]);
     if constexpr (BITS == 32) {
-      rm[u] = ((const float4*)first_)[at / 4];
-      rv[u] = ((const float4*)second_)[at / 4];
+      rm[u] = ((const float4*)first_)[i / 4];
+      rv[u] = ((const float4*)second_)[i / 4];
     } else {
-      cm[u] = ((const uint32_t*)first_)[at / 4];
-      cr[u] = ((const uint32_t*)second_)[at / 4];
-      em[u] = first_e[at / BLOCK];
-      er[u] = second_e[at / BLOCK];
+      cm[u] = ((const uint32_t*)first_)[i / 4];
+      cr[u] = ((const uint32_t*)second_)[i / 4];
+      em[u] = first_e[i / BLOCK];
+      er[u] = second_e[i / BLOCK];
     }
   }
 #pragma unroll
   for (int u = 0; u < TURNS; ++u) {
-    const int64_t i = begin + 1024 * u + 4 * threadIdx.x;
-    if (i >= padded) continue;
-    const int64_t at = T.offset + i;
+    const int i = 1024 * u + 4 * threadIdx.x;
+    if (!FULL && i >= padded) continue;
     float p[4], g[4], m[4], root[4];
-    as_floats(T.type, rp[u], p);
+    as_floats(pt, rp[u], p);
     as_floats(gt, rg[u], g);
     if constexpr (BITS == 32) {
       m[0] = rm[u].x; m[1] = rm[u].y; m[2] = rm[u].z; m[3] = rm[u].w;
       float v[4] = {rv[u].x, rv[u].y, rv[u].z, rv[u].w};
-      const float b1 = (float)beta1, c1 = (float)(1.0 - beta1), b2 = (float)beta2, c2 = (float)(1.0 - beta2);
+      const float b1 = (float)rate.beta1, c1 = (float)(1.0 - rate.beta1), b2 = (float)rate.beta2, c2 = (float)(1.0 - rate.beta2);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float gk = g[k] * gs;
@@ -189,8 +180,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(const rlgan_adamw_tensor_t* 
         v[k] = v[k] * b2 + gk * c2 * gk;
         root[k] = sqrtf(v[k]);
       }
-      ((float4*)first_)[at / 4] = make_float4(m[0], m[1], m[2], m[3]);
-      ((float4*)second_)[at / 4] = make_float4(v[0], v[1], v[2], v[3]);
+      ((float4*)first_)[i / 4] = make_float4(m[0], m[1], m[2], m[3]);
+      ((float4*)second_)[i / 4] = make_float4(v[0], v[1], v[2], v[3]);
     } else {
       // Codes are decided by 64-bit arithmetic, without contraction: b1 m + (1 - b1) g of values with so few bits lands on the border
       // between two codes often enough (15 * 0.9 = 13.5), and 32 bits would decide by their own rounding there.  The root's are
@@ -201,11 +192,11 @@ __global__ __launch_bounds__(256) void adamw_kernel(const rlgan_adamw_tensor_t* 
       decode4(cm[u], em[u], cr[u], er[u], m, root);
       double dm[4];
       int rr[4];
-      const float b2 = (float)beta2, c2 = (float)(1.0 - beta2);
+      const float b2 = (float)rate.beta2, c2 = (float)(1.0 - rate.beta2);
       bool unsure = false;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        dm[k] = (double)m[k] * beta1 + (double)g[k] * (double)gs * (1.0 - beta1);
+        dm[k] = (double)m[k] * rate.beta1 + (double)g[k] * (double)gs * (1.0 - rate.beta1);
         m[k] = (float)dm[k];
         const float gk = g[k] * gs, v = root[k] * root[k] * b2 + gk * c2 * gk, s = __builtin_amdgcn_sqrtf(v);
         rr[k] = v == 0.f ? 0 : Root::rounded(s, 16);
@@ -218,7 +209,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const rlgan_adamw_tensor_t* 
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (rr[k] >= 0) continue;
-          const double gk = (double)g[k] * (double)gs, r = root[k], s = sqrt(r * r * beta2 + gk * (1.0 - beta2) * gk);
+          const double gk = (double)g[k] * (double)gs, r = root[k], s = sqrt(r * r * rate.beta2 + gk * (1.0 - rate.beta2) * gk);
           rr[k] = Root::rounded(s);
           root[k] = (float)s;
         }
@@ -226,14 +217,33 @@ __global__ __launch_bounds__(256) void adamw_kernel(const rlgan_adamw_tensor_t* 
       uint32_t nm, nr;
       int fm, fr;
       encode4(dm, rr, nm, fm, nr, fr);
-      ((uint32_t*)first_)[at / 4] = nm;
-      ((uint32_t*)second_)[at / 4] = nr;
-      if ((threadIdx.x & 15) == 0) { first_e[at / BLOCK] = (uint8_t)fm; second_e[at / BLOCK] = (uint8_t)fr; }
+      ((uint32_t*)first_)[i / 4] = nm;
+      ((uint32_t*)second_)[i / 4] = nr;
+      if ((threadIdx.x & 15) == 0) { first_e[i / BLOCK] = (uint8_t)fm; second_e[i / BLOCK] = (uint8_t)fr; }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) p[k] = p[k] * sc.keep - sc.lr_t * m[k] * __builtin_amdgcn_rcpf(root[k] * sc.root_t + eps);
-    RLGAN_BY_TYPE(T.type, E, store4<E>(T.param, i, T.count, p));
+    for (int k = 0; k < 4; ++k) p[k] = p[k] * sc.keep - sc.lr_t * m[k] * __builtin_amdgcn_rcpf(root[k] * sc.root_t + rate.eps);
+    RLGAN_BY_TYPE(pt, E, store4<FULL, E>(pp, begin, i, n, p));
   }
+}
+
+template <int BITS>
+__global__ __launch_bounds__(256) void adamw_kernel(const rlgan_adamw_tensor_t* tensors, const int32_t* chunks, int64_t chunk0, int tensor0,
+                                                    Grads grads, void* first, void* second, uint8_t* first_e, uint8_t* second_e,
+                                                    double beta1, double beta2, float eps, const float* grad_scale, const Scalars* scalars) {
+  const Scalars sc = *scalars;
+  if (sc.skip) return;
+  const int ti = chunks[2 * (chunk0 + blockIdx.x)], ci = chunks[2 * (chunk0 + blockIdx.x) + 1];
+  const rlgan_adamw_tensor_t T = tensors[ti];
+  const void* gp = grads.p[ti - tensor0];
+  const int gt = grads.type[ti - tensor0];
+  const Rates rate{beta1, beta2, eps, grad_scale ? *grad_scale : 1.f};
+  const int64_t begin = (int64_t)ci * CHUNK, at = T.offset + begin;
+  constexpr int SIZE = BITS / 8;
+  void* f = (char*)first + at * SIZE; void* s = (char*)second + at * SIZE;
+  uint8_t* fe = BITS == 8 ? first_e + at / BLOCK : nullptr; uint8_t* se = BITS == 8 ? second_e + at / BLOCK : nullptr;
+  if (begin + CHUNK <= T.count) adamw_chunk<BITS, true>(T.type, T.param, gt, gp, begin, CHUNK, f, s, fe, se, rate, sc);
+  else adamw_chunk<BITS, false>(T.type, T.param, gt, gp, begin, (int)(T.count - begin), f, s, fe, se, rate, sc);
 }
 
 // 8-bit states as 32-bit numbers, and back
