@@ -112,6 +112,9 @@ __global__ __launch_bounds__(256) void scan_serial_bwd(Units u, Seq<const T> dh,
 // composition of the maps before it.
 
 constexpr int WAVES = 8, STEPS = 8, TILE = WAVES * STEPS;
+// the backward walk has twice the tensors to hold: 4 steps a wave leave room for two workgroups a CU (16385 steps of 3000 units bf16
+// 143 us; 8 steps 157)
+constexpr int BACK_STEPS = 4, BACK_TILE = WAVES * BACK_STEPS;
 
 // h -> a h + b; a < 0 (by its sign bit, which products with f keep): the state from before does not reach through, h -> b
 struct Map { float a, b; };
@@ -121,13 +124,24 @@ __device__ __forceinline__ Map compose(Map late, Map early) {
 }
 constexpr float DROP = -1.f;
 
+// Where a workgroup works.  Workgroups go to the 8 XCDs in turn.  Where a row's tiles meet inside a cache line and the time axis is
+// whole, neighbouring tiles are given to one XCD, a run of workgroups to each (`runs`): backward of 129 x 200 fp32 units over 200
+// steps 35.8 us, 40.2 in the plain order.  Where they meet between lines or segments lie far apart the plain order is better
+// (backward walk of 3 x 1000 bf16 units in 22 segments 150 us, in runs 177).
+struct Place { int tile, segment; };
+__device__ __forceinline__ Place place(int tiles, bool runs) {
+  const int total = gridDim.x, id = blockIdx.x, xcd = id % 8, share = total / 8, rest = total % 8;
+  const int k = runs ? xcd * share + min(xcd, rest) + id / 8 : id;
+  return {k % tiles, k / tiles};
+}
+
 template <int VEC> struct Lanes {                // the units of a lane
   int64_t unit;                                  // first of them, counted through the batch
   int b, d, len;
   bool real;
-  __device__ __forceinline__ Lanes(const Units& u, bool mask) {
+  __device__ __forceinline__ Lanes(const Units& u, int tile, bool mask) {
     const int wv = u.width / VEC, total = u.batch * wv;
-    const int i = blockIdx.x * 64 + (threadIdx.x & 63), k = min(i, total - 1);   // lanes behind the last repeat it and write nothing
+    const int i = tile * 64 + (threadIdx.x & 63), k = min(i, total - 1);   // lanes behind the last repeat it and write nothing
     real = i < total;
     b = k / wv; d = (k - b * wv) * VEC;
     unit = (int64_t)b * u.width + d;
@@ -136,16 +150,16 @@ template <int VEC> struct Lanes {                // the units of a lane
 };
 
 // STEPS steps from `t0` on of one sequence tensor; steps behind the end of the axis repeat its last one
-template <typename T, int VEC>
-__device__ __forceinline__ void load_steps(Vec<T, VEC> (&v)[STEPS], const T* p, int64_t stride, int t0, int length) {
+template <typename T, int VEC, int COUNT>
+__device__ __forceinline__ void load_steps(Words<T, VEC> (&v)[COUNT], const T* p, int64_t stride, int t0, int length) {
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i) v[i].load(p + min(max(t0 + i, 0), length - 1) * stride);
+  for (int i = 0; i < COUNT; ++i) v[i].load(p + min(max(t0 + i, 0), length - 1) * stride);
 }
-__device__ __forceinline__ uint32_t load_starts(const uint8_t* p, int64_t stride, int t0, int length) {
+template <int COUNT = STEPS> __device__ __forceinline__ uint32_t load_starts(const uint8_t* p, int64_t stride, int t0, int length) {
   uint32_t bits = 0;
   if (p) {
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) bits |= (p[min(t0 + i, length - 1) * stride] ? 1u : 0u) << i;
+    for (int i = 0; i < COUNT; ++i) bits |= (p[min(t0 + i, length - 1) * stride] ? 1u : 0u) << i;
   }
   return bits;
 }
@@ -161,15 +175,16 @@ __device__ __forceinline__ void fold_backward(Map& m, float f, float dh, bool st
   m = live ? Map{a, b} : m;
 }
 
-struct Cut { int segment, segments; Map* maps; };    // steps a segment (a multiple of TILE); maps[slot][unit]
+struct Cut { int tiles, segment, segments; bool runs; Map* maps; };    // segment: steps a segment (a multiple of TILE); maps[slot][unit]
 
-// One segment's map.  Forward: slot blockIdx.y + 1 holds segment blockIdx.y, slot 0 the state handed in; backward: slot s of
+// One segment's map.  Forward: slot s + 1 holds segment s, slot 0 the state handed in; backward: slot s of
 // segments + 1 holds segment s (s >= 1), the last one the gradient handed in.
 template <typename T, int VEC, bool MASK, bool BACK>
 __global__ __launch_bounds__(WAVES * 64) void scan_fold_kernel(Units u, Seq<const T> z, Seq<const T> x_or_dh, const float* handed, Cut cut) {
   __shared__ Map sh[WAVES][64 * VEC];
-  const Lanes<VEC> me(u, MASK);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, seg = BACK ? blockIdx.y + 1 : blockIdx.y;
+  const Place at = place(cut.tiles, false);
+  const Lanes<VEC> me(u, at.tile, MASK);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, seg = BACK ? at.segment + 1 : at.segment;
   const int64_t units = (int64_t)u.batch * u.width;
   const int per_wave = cut.segment / WAVES, begin = seg * cut.segment + wave * per_wave, end = min(begin + per_wave, u.length);
   const T* zp = z.p + me.b * z.b + me.d; const T* xp = x_or_dh.p + me.b * x_or_dh.b + me.d;
@@ -177,7 +192,7 @@ __global__ __launch_bounds__(WAVES * 64) void scan_fold_kernel(Units u, Seq<cons
   Map m[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) m[k] = {1.f, 0.f};
-  Vec<T, VEC> zv[2][STEPS], xv[2][STEPS];
+  Words<T, VEC> zv[2][STEPS], xv[2][STEPS];
   uint32_t st[2] = {0, 0};
   const int n = end > begin ? (end - begin + STEPS - 1) / STEPS : 0;
   const int first = BACK ? begin + (n - 1) * STEPS : begin, hop = BACK ? -STEPS : STEPS;
@@ -251,14 +266,15 @@ __device__ __forceinline__ void enter_segment(const Lanes<VEC>& me, const Cut& c
 template <typename T, int VEC, bool MASK>
 __global__ __launch_bounds__(WAVES * 64) void scan_walk_fwd(Units u, Seq<const T> z, Seq<const T> x, Seq<T> h, float* state_out, Cut cut) {
   __shared__ Map sh[2][WAVES][64 * VEC];
-  const Lanes<VEC> me(u, MASK);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, seg = blockIdx.y;
+  const Place at = place(cut.tiles, cut.runs);
+  const Lanes<VEC> me(u, at.tile, MASK);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, seg = at.segment;
   const int64_t units = (int64_t)u.batch * u.width;
   const T* zp = z.p + me.b * z.b + me.d; const T* xp = x.p + me.b * x.b + me.d; T* hp = h.p + me.b * h.b + me.d;
   const uint8_t* sp = MASK && u.starts ? u.starts + me.b * u.starts_b : nullptr;
   float s[VEC];
   const int begin = seg * cut.segment, end = min(begin + cut.segment, u.length);
-  Vec<T, VEC> zn[STEPS], xn[STEPS];
+  Words<T, VEC> zn[STEPS], xn[STEPS];
   load_steps(zn, zp, z.t, begin + wave * STEPS, u.length);
   load_steps(xn, xp, x.t, begin + wave * STEPS, u.length);
   uint32_t stn = load_starts(sp, u.starts_t, begin + wave * STEPS, u.length);
@@ -324,11 +340,12 @@ __global__ __launch_bounds__(WAVES * 64) void scan_walk_fwd(Units u, Seq<const T
 }
 
 template <typename T, int VEC, bool MASK>
-__global__ __launch_bounds__(WAVES * 64) void scan_walk_bwd(Units u, Seq<const T> dh, Seq<const T> z, Seq<const T> x, Seq<const T> h,
+__global__ __launch_bounds__(WAVES * 64, 4) void scan_walk_bwd(Units u, Seq<const T> dh, Seq<const T> z, Seq<const T> x, Seq<const T> h,
                                                             const float* dstate, Seq<T> dz, Seq<T> dx, float* dstate_in, Cut cut) {
   __shared__ Map sh[2][WAVES][64 * VEC];
-  const Lanes<VEC> me(u, MASK);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, seg = blockIdx.y;
+  const Place at = place(cut.tiles, cut.runs);
+  const Lanes<VEC> me(u, at.tile, MASK);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, seg = at.segment;
   const int64_t units = (int64_t)u.batch * u.width;
   const T* gp = dh.p + me.b * dh.b + me.d; const T* zp = z.p + me.b * z.b + me.d;
   const T* xp = x.p + me.b * x.b + me.d; const T* hp = h.p + me.b * h.b + me.d;
@@ -336,41 +353,41 @@ __global__ __launch_bounds__(WAVES * 64) void scan_walk_bwd(Units u, Seq<const T
   const uint8_t* sp = MASK && u.starts ? u.starts + me.b * u.starts_b : nullptr;
   float c[VEC];
   const int begin = seg * cut.segment, end = min(begin + cut.segment, u.length);
-  const int last = begin + (end - begin - 1) / TILE * TILE;
-  Vec<T, VEC> zn[STEPS], xn[STEPS], gn[STEPS], hn[STEPS];
+  const int last = begin + (end - begin - 1) / BACK_TILE * BACK_TILE;
+  Words<T, VEC> zn[BACK_STEPS], xn[BACK_STEPS], gn[BACK_STEPS], hn[BACK_STEPS];
   uint32_t stn;
   auto fetch = [&](int t0) {
     load_steps(zn, zp, z.t, t0, u.length);
     load_steps(gn, gp, dh.t, t0, u.length);
     load_steps(xn, xp, x.t, t0, u.length);
     load_steps(hn, hp, h.t, t0 - 1, u.length);
-    stn = load_starts(sp, u.starts_t, t0, u.length);
+    stn = load_starts<BACK_STEPS>(sp, u.starts_t, t0, u.length);
   };
-  fetch(last + wave * STEPS);
+  fetch(last + wave * BACK_STEPS);
   if (cut.segments > 1) enter_segment<VEC, true>(me, cut, seg, units, sh[0], c);
   else {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) c[k] = dstate ? dstate[me.unit + k] : 0.f;
   }
   int turn = 0;
-  for (int tile = last; tile >= begin; tile -= TILE, turn ^= 1) {
-    const int t0 = tile + wave * STEPS;
-    float f[STEPS][VEC], take[STEPS][VEC];
-    Vec<T, VEC> xv[STEPS], gv[STEPS], hv[STEPS];
+  for (int tile = last; tile >= begin; tile -= BACK_TILE, turn ^= 1) {
+    const int t0 = tile + wave * BACK_STEPS;
+    Words<T, VEC> xv[BACK_STEPS], gv[BACK_STEPS], hv[BACK_STEPS];
     const uint32_t st = stn;
+    float fs[BACK_STEPS][VEC], takes[BACK_STEPS][VEC];
     Map m[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) m[k] = {1.f, 0.f};
 #pragma unroll
-    for (int i = STEPS - 1; i >= 0; --i) {
+    for (int i = BACK_STEPS - 1; i >= 0; --i) {
       xv[i] = xn[i]; gv[i] = gn[i]; hv[i] = hn[i];
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
-        gate(zn[i].get(k), f[i][k], take[i][k]);
-        fold_backward(m[k], f[i][k], gv[i].get(k), MASK && ((st >> i) & 1), t0 + i < me.len);
+        gate(zn[i].get(k), fs[i][k], takes[i][k]);
+        fold_backward(m[k], fs[i][k], gv[i].get(k), MASK && ((st >> i) & 1), t0 + i < me.len);
       }
     }
-    if (tile > begin) fetch(t0 - TILE);
+    if (tile > begin) fetch(t0 - BACK_TILE);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) sh[turn][wave][lane * VEC + k] = m[k];
     __syncthreads();
@@ -386,17 +403,18 @@ __global__ __launch_bounds__(WAVES * 64) void scan_walk_bwd(Units u, Seq<const T
       c[k] = v;
     }
 #pragma unroll
-    for (int i = STEPS - 1; i >= 0; --i) {
+    for (int i = BACK_STEPS - 1; i >= 0; --i) {
       if (t0 + i >= u.length) continue;
       Vec<T, VEC> oz, ox;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         const bool live = !MASK || t0 + i < me.len, start = MASK && ((st >> i) & 1);
         const float before = t0 + i > 0 ? hv[i].get(k) : u.state ? u.state[me.unit + k] : 0.f, p = start ? 0.f : before;
-        const float g = mine[k] + gv[i].get(k), gt = g * take[i][k];
+        const float f = fs[i][k], take = takes[i][k];
+        const float g = mine[k] + gv[i].get(k), gt = g * take;
         ox.set(k, live ? gt : 0.f);
-        oz.set(k, live ? gt * f[i][k] * (p - xv[i].get(k)) : 0.f);
-        mine[k] = live ? (start ? 0.f : f[i][k] * g) : mine[k];
+        oz.set(k, live ? gt * f * (p - xv[i].get(k)) : 0.f);
+        mine[k] = live ? (start ? 0.f : f * g) : mine[k];
       }
       if (me.real) { oz.store(ozp + (t0 + i) * dz.t); ox.store(oxp + (t0 + i) * dx.t); }
     }
@@ -412,19 +430,20 @@ __global__ __launch_bounds__(WAVES * 64) void scan_walk_bwd(Units u, Seq<const T
 // Up to SERIAL steps one thread a unit is best (a single step is one read and one write); behind that the tiled form.
 constexpr int SERIAL = 8;
 
-struct Plan { bool serial; int vec, tiles; Cut cut; };
+struct Plan { bool serial; int vec; Cut cut; };
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // A cut costs a second read of two tensors, idle CUs cost bandwidth.  Measured on an MI355X with 256, 512, 1024, 2048 workgroups
 // wanted: 65536 steps of 512 units forward fp32 161, 145, 149, 154 us, 16385 of 3000 backward bf16 257, 223, 231, 237; and with 256 or
 // more workgroups of units (1024 steps of 32768 units bf16: 46 us) a cut loses (70 us in two segments).
-inline Plan plan(int batch, int length, int width, int vec) {
+inline Plan plan(int batch, int length, int width, int size, int vec) {
   constexpr int WANT = 512;
-  Plan p{length <= SERIAL, vec, (int)cdiv((int64_t)batch * (width / vec), 64), {}};
-  const int64_t segments = p.tiles >= WANT / 2 ? 1 : cdiv(WANT, p.tiles), steps = cdiv(cdiv(length, segments), TILE) * TILE;
+  Plan p{length <= SERIAL, vec, {(int)cdiv((int64_t)batch * (width / vec), 64), 0, 0, false, nullptr}};
+  const int64_t segments = p.cut.tiles >= WANT / 2 ? 1 : cdiv(WANT, p.cut.tiles), steps = cdiv(cdiv(length, segments), TILE) * TILE;
   p.cut.segment = (int)steps;
   p.cut.segments = (int)cdiv(length, steps);
+  p.cut.runs = p.cut.segments == 1 && width * size % 128 != 0;
   return p;
 }
 
@@ -475,7 +494,7 @@ int rlgan_gated_scan_workspace(int batch, int length, int width, int type, int b
   int64_t most = 0;                              // one or two units a lane: the call decides by its tensors' alignment
   for (int vec = 1; vec <= 2; ++vec) {
     if (width % vec) break;
-    const Plan p = plan(batch, length, width, vec);
+    const Plan p = plan(batch, length, width, type == TYPE_F32 ? 4 : 2, vec);
     if (!p.serial && p.cut.segments > 1) most = std::max(most, (int64_t)(p.cut.segments + 1) * batch * width * (int64_t)sizeof(Map));
   }
   *bytes = most;
@@ -487,7 +506,7 @@ int rlgan_gated_scan_forward(const rlgan_scan_t* s, rlgan_seq_t h, float* state_
   if (!h.p || !state_out) return RLGAN_E_ARG;
   const Units u = units(s);
   const bool mask = s->starts || s->lengths;
-  Plan p = plan(s->batch, s->length, s->width, vec_of(s, {s->z, s->x, h}));
+  Plan p = plan(s->batch, s->length, s->width, s->type == TYPE_F32 ? 4 : 2, vec_of(s, {s->z, s->x, h}));
   p.cut.maps = (Map*)workspace;
   hipStream_t st = (hipStream_t)stream;
   if (p.serial) {
@@ -497,10 +516,10 @@ int rlgan_gated_scan_forward(const rlgan_scan_t* s, rlgan_seq_t h, float* state_
   }
   if (p.cut.segments > 1) {
     if (!workspace) return RLGAN_E_ARG;
-    RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_fold_kernel<T, VEC, MASK, false>), dim3(p.tiles, p.cut.segments - 1), dim3(WAVES * 64), 0, st, u,
+    RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_fold_kernel<T, VEC, MASK, false>), dim3(p.cut.tiles * (p.cut.segments - 1)), dim3(WAVES * 64), 0, st, u,
                                           in<T>(s->z), in<T>(s->x), s->state, p.cut));
   }
-  RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_walk_fwd<T, VEC, MASK>), dim3(p.tiles, p.cut.segments), dim3(WAVES * 64), 0, st, u, in<T>(s->z),
+  RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_walk_fwd<T, VEC, MASK>), dim3(p.cut.tiles * p.cut.segments), dim3(WAVES * 64), 0, st, u, in<T>(s->z),
                                         in<T>(s->x), out<T>(h), state_out, p.cut));
   return (int)hipGetLastError();
 }
@@ -518,7 +537,7 @@ int rlgan_gated_scan_backward(const rlgan_scan_t* s, rlgan_seq_t h, rlgan_seq_t 
   if (!h.p || !dh.p || !dz.p || !dx.p || !dstate_in) return RLGAN_E_ARG;
   const Units u = units(s);
   const bool mask = s->starts || s->lengths;
-  Plan p = plan(s->batch, s->length, s->width, vec_of(s, {s->z, s->x, h, dh, dz, dx}));
+  Plan p = plan(s->batch, s->length, s->width, s->type == TYPE_F32 ? 4 : 2, vec_of(s, {s->z, s->x, h, dh, dz, dx}));
   p.cut.maps = (Map*)workspace;
   hipStream_t st = (hipStream_t)stream;
   if (p.serial) {
@@ -529,10 +548,10 @@ int rlgan_gated_scan_backward(const rlgan_scan_t* s, rlgan_seq_t h, rlgan_seq_t 
   }
   if (p.cut.segments > 1) {
     if (!workspace) return RLGAN_E_ARG;
-    RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_fold_kernel<T, VEC, MASK, true>), dim3(p.tiles, p.cut.segments - 1), dim3(WAVES * 64), 0, st, u,
+    RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_fold_kernel<T, VEC, MASK, true>), dim3(p.cut.tiles * (p.cut.segments - 1)), dim3(WAVES * 64), 0, st, u,
                                           in<T>(s->z), in<T>(dh), dstate, p.cut));
   }
-  RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_walk_bwd<T, VEC, MASK>), dim3(p.tiles, p.cut.segments), dim3(WAVES * 64), 0, st, u, in<T>(dh),
+  RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_walk_bwd<T, VEC, MASK>), dim3(p.cut.tiles * p.cut.segments), dim3(WAVES * 64), 0, st, u, in<T>(dh),
                                         in<T>(s->z), in<T>(s->x), in<T>(h), dstate, out<T>(dz), out<T>(dx), dstate_in, p.cut));
   return (int)hipGetLastError();
 }

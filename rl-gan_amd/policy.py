@@ -4,6 +4,7 @@ pass over the logits.  For policies over discrete actions (or tokens), beside th
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -79,10 +80,8 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logp: torch.Ten
         none = torch.zeros(0, dtype=torch.float32, device=dev)
         return PolicyLoss(torch.zeros((), dtype=torch.float32, device=dev), none, none.clone(), none.clone(), d)
     with guard(dev):
-        size = C.c_int64()
-        check(lib.rlgan_policy_loss_workspace(rows, vocab, code, C.byref(size)), "rlgan_policy_loss_workspace")
         # the workspace (8-byte sums in front), then the three rows of results: one allocation of this call alone
-        words = (size.value + 3) // 4
+        words = (_workspace_bytes(rows, vocab, code) + 3) // 4
         room = torch.empty(words + 3 * rows, dtype=torch.float32, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev)
         base = room.data_ptr()
@@ -93,6 +92,13 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logp: torch.Ten
         check(lib.rlgan_policy_loss(C.byref(args), base, stream_of(dev)), "rlgan_policy_loss")
     _, logp, entropy, kl = room.split([words, rows, rows, rows])
     return PolicyLoss(loss, logp, entropy, kl, d)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(rows: int, vocab: int, code: int) -> int:
+    size = C.c_int64()
+    check(lib.rlgan_policy_loss_workspace(rows, vocab, code, C.byref(size)), "rlgan_policy_loss_workspace")
+    return size.value
 
 
 def _row_stride(t: torch.Tensor, vocab: int) -> int:

@@ -10,6 +10,7 @@ and any other strides (time-major data goes in as a transposed view, the two hal
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional, Tuple
 
 import numpy as np
@@ -20,20 +21,21 @@ from .conv import DenseLayer
 from .tensors import apart, byte_range, first_device, guard, need, on_device, stream_of, type_code, vector, workspace
 
 
-def _seq(t: torch.Tensor, shape, dtype, dev, name: str) -> SeqRef:
-    on_device(t, dev, name)
-    if t.dtype != dtype or t.shape != shape:
+def _seq(t: torch.Tensor, shape, dtype, dev: torch.device, name: str) -> SeqRef:
+    if t.get_device() != dev.index or t.dtype != dtype or t.shape != shape:
+        on_device(t, dev, name)
         raise ValueError(f"{name}: {dtype} of shape {tuple(shape)} is wanted, got {t.dtype} {tuple(t.shape)}")
-    if t.stride(2) != 1 and shape[2] > 1:
+    b, n, c = t.stride()
+    if c != 1 and shape[2] > 1:
         raise ValueError(f"{name}: channels have to lie next to each other (strides {t.stride()})")
-    return SeqRef(t.data_ptr(), t.stride(0), t.stride(1))
+    return SeqRef(t.data_ptr(), b, n)
 
 
 def _scan(z, x, state, starts, lengths) -> Tuple[Scan, torch.device]:
     dev = first_device(z, "z")
     code = type_code(z, "z")
-    need(z.dim() == 3, "z and x are [batch, time, width]")
-    shape = z.shape
+    shape, dtype = z.shape, z.dtype
+    need(len(shape) == 3, "z and x are [batch, time, width]")
     b, n, d = shape
     need(b * d <= 1 << 31 and n < 1 << 31, "at most 2^31 units and steps")
     st = None
@@ -41,8 +43,8 @@ def _scan(z, x, state, starts, lengths) -> Tuple[Scan, torch.device]:
     if starts is not None:
         on_device(starts, dev, "starts")
         need(starts.dtype in (torch.bool, torch.uint8) and starts.shape == shape[:2], "starts: bool or uint8 of shape [batch, time]")
-        st, sb, ss = starts.data_ptr(), starts.stride(0), starts.stride(1)
-    return Scan(b, n, d, code, _seq(z, shape, z.dtype, dev, "z"), _seq(x, shape, z.dtype, dev, "x"), vector(state, (b, d), dev, "state"), st,
+        st, (sb, ss) = starts.data_ptr(), starts.stride()
+    return Scan(b, n, d, code, _seq(z, shape, dtype, dev, "z"), _seq(x, shape, dtype, dev, "x"), vector(state, (b, d), dev, "state"), st,
                 sb, ss, vector(lengths, (b,), dev, "lengths", torch.int32)), dev
 
 
@@ -53,10 +55,15 @@ def _output(out, like, others, name):
     return out
 
 
-def _workspace(s: Scan, backward: int, dev) -> Optional[torch.Tensor]:
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(batch: int, length: int, width: int, code: int, backward: int) -> int:
     size = C.c_int64()
-    check(lib.rlgan_gated_scan_workspace(s.batch, s.length, s.width, s.type, backward, C.byref(size)), "rlgan_gated_scan_workspace")
-    return workspace(size.value, dev)
+    check(lib.rlgan_gated_scan_workspace(batch, length, width, code, backward, C.byref(size)), "rlgan_gated_scan_workspace")
+    return size.value
+
+
+def _workspace(s: Scan, backward: int, dev) -> Optional[torch.Tensor]:
+    return workspace(_workspace_bytes(s.batch, s.length, s.width, s.type, backward), dev)
 
 
 def gated_scan(z: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tensor] = None, *, starts: Optional[torch.Tensor] = None,

@@ -25,7 +25,7 @@ def type_code(t: torch.Tensor, name: str) -> int:
 
 
 def on_device(t: torch.Tensor, dev: torch.device, name: str) -> None:
-    if not t.is_cuda or t.device != dev:
+    if t.get_device() != dev.index:                             # -1 for a CPU tensor
         raise ValueError(f"{name} is on {t.device}: the call's tensors are on {dev}, an AMD GPU")
 
 
@@ -40,7 +40,7 @@ def vector(t: Optional[torch.Tensor], shape, dev: torch.device, name: str, dtype
     if t is None:
         return None
     on_device(t, dev, name)
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} is wanted, got {t.dtype} {tuple(t.shape)} "
                          f"with strides {t.stride()}")
     return t.data_ptr()
