@@ -710,8 +710,9 @@ int rlgan_policy_loss(const rlgan_policy_t* p, void* workspace, void* stream);
  * finite reads as NaN.
  * chunks: device, (tensor, chunk of RLGAN_ADAMW_CHUNK elements within it) for every chunk of every tensor in order; chunk_begin:
  * HOST, n_tensors + 1 places of the tensors' first chunks.  step: device counter of the steps done, advanced by the call; lr:
- * device scalar; scalars: device scratch of 16 bytes. */
+ * device scalar; scalars: device scratch of RLGAN_ADAMW_SCALARS bytes. */
 #define RLGAN_ADAMW_CHUNK 2048
+#define RLGAN_ADAMW_SCALARS 32
 typedef struct { void* param; int64_t count, offset; int32_t type, reserved; } rlgan_adamw_tensor_t;
 typedef struct {
   int32_t n_tensors, state_bits;
@@ -724,6 +725,8 @@ typedef struct {
   int32_t* step;
   float* scalars;
   double beta1, beta2, eps, weight_decay;
+  int32_t random, reserved;                /* 8 bits: codes rounded at random (1), by Philox under `seed`, or to nearest (0) */
+  uint64_t seed;
 } rlgan_adamw_t;
 /* grads, grad_types: HOST arrays of n_tensors device pointers and element types (any of the three, whatever the parameter's).
  * grad_scale: device scalar or NULL.  skip: device byte or NULL; where it is not 0 the call changes nothing. */

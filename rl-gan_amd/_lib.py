@@ -167,7 +167,8 @@ class AdamWTensor(C.Structure):
 class AdamWState(C.Structure):
     _fields_ = [("n_tensors", _i32), ("state_bits", _i32), ("tensors", _fp), ("chunks", _fp), ("chunk_begin", _fp), ("first", _fp),
                 ("second", _fp), ("first_exp", _fp), ("second_exp", _fp), ("lr", _fp), ("step", _fp), ("scalars", _fp),
-                ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double)]
+                ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double), ("random", _i32),
+                ("reserved", _i32), ("seed", C.c_uint64)]
 
 
 def _load():

@@ -21,13 +21,19 @@ class AdamW:
     computed in float32 and rounded to the parameter's type (to nearest: 16-bit weights lose updates below half a step).
     state_bits 32: moments as float32, 8 bytes a parameter.  state_bits 8: one byte each for m and the root of v, 2.03 bytes a
     parameter; every 64 elements share an exponent under which codes reach 16 octaves, rounded by at most 2^-4 (m) and 2^-5 (root).
+    rounding "nearest" of the 8-bit codes loses what a step changes by less than half a code: at betas[1] = 0.999 a second moment
+    rises only where a gradient exceeds its root some 6 times and never falls, which suits a few hundred steps (fine-tuning,
+    tests) and no more.  "random" rounds up with the probability of the part cut off (Philox under `seed`, counted by step and
+    element, so a run repeats to the bit): the moments follow in the mean, for training of any length.
     `lr` and `steps` are device scalars that the kernels read, so that a captured step follows `set_lr` and counts on."""
 
     def __init__(self, params: Sequence[torch.Tensor], lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
-                 weight_decay: float = 1e-2, state_bits: int = 32):
+                 weight_decay: float = 1e-2, state_bits: int = 32, rounding: str = "nearest", seed: int = 0):
         self.params: List[torch.Tensor] = list(params)
         need(len(self.params) > 0, "no parameters")
         need(state_bits in (8, 32), "state_bits: 8 or 32")
+        need(rounding in ("nearest", "random"), "rounding: \"nearest\" or \"random\"")
+        need(0 <= int(seed) < 1 << 64, "seed: an unsigned 64-bit number")
         need(0 <= betas[0] < 1 and 0 <= betas[1] < 1, "betas: at least 0 and below 1")
         need(lr >= 0 and eps >= 0 and weight_decay >= 0, "lr, eps and weight_decay: not negative")
         self.device = dev = first_device(self.params[0], "params[0]")
@@ -63,11 +69,11 @@ class AdamW:
             self.second_exp = torch.zeros_like(self.first_exp)
         self.lr = torch.full((1,), float(lr), dtype=torch.float32, device=dev)
         self.steps = torch.zeros(1, dtype=torch.int32, device=dev)
-        self._scalars = torch.zeros(4, dtype=torch.float32, device=dev)
+        self._scalars = torch.zeros(8, dtype=torch.float32, device=dev)
         ptr = lambda t: None if t is None else t.data_ptr()
         self._state = AdamWState(len(counts), state_bits, ptr(self._records), ptr(self._chunks), self._chunk_begin.ctypes.data, ptr(self.first),
                                  ptr(self.second), ptr(self.first_exp), ptr(self.second_exp), ptr(self.lr), ptr(self.steps), ptr(self._scalars),
-                                 self.betas[0], self.betas[1], self.eps, self.weight_decay)
+                                 self.betas[0], self.betas[1], self.eps, self.weight_decay, rounding == "random", 0, int(seed))
 
     def set_lr(self, lr: float) -> None:
         """The rate of the following steps, those of captured graphs among them."""

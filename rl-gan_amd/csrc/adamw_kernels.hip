@@ -6,6 +6,7 @@
 // in a floating code and makes decoding exact.  A magnitude under the range becomes 0 in m but the smallest code in the root,
 // so that no step divides by eps alone what was small.  gfx950 only.
 #include "rlgan_types.h"
+#include "rlgan_rng.h"
 #include "rlgan_host.h"
 
 using namespace rlgan;
@@ -18,7 +19,8 @@ constexpr int GROUP = 384;                      // tensors of a launch: their gr
 
 struct Grads { const void* p[GROUP]; uint8_t type[GROUP]; };
 
-struct Scalars { float lr_t, root_t, keep; int skip; };
+struct Scalars { float lr_t, root_t, keep; int32_t skip, step; };
+static_assert(sizeof(Scalars) <= RLGAN_ADAMW_SCALARS, "the caller's scratch holds it");
 
 __global__ void adamw_begin_kernel(int32_t* step, const float* lr, double beta1, double beta2, double decay, const uint8_t* skip, Scalars* out) {
   const bool no = skip && *skip;
@@ -29,6 +31,7 @@ __global__ void adamw_begin_kernel(int32_t* step, const float* lr, double beta1,
   out->root_t = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t)));
   out->keep = (float)(1.0 - rate * decay);
   out->skip = no;
+  out->step = t;
 }
 
 // 4 elements from the i-th on as they lie in memory, and as floats: apart, so that a workgroup's loads are all in flight before the
@@ -83,7 +86,13 @@ template <int MAN, int COUNT> struct Small {
     const int u = (int)((h + ((1u << (19 - MAN)) - 1) + ((h >> (20 - MAN)) & 1)) >> (20 - MAN)) - (896 << MAN);
     return u < (1 << MAN) ? 0 : min(u, 255 << MAN);
   }
-  // the same of a normal float that is known to `slack` units of its last place; -1 where that does not decide
+  // rounded up with the probability of what is cut off, by 16 random bits
+  static __device__ __forceinline__ int rounded(double v, uint32_t random16) {
+    const uint32_t h = (uint32_t)((uint64_t)__double_as_longlong(v) >> 32) & 0x7FFFFFFFu;
+    const int u = (int)((h + (random16 << (4 - MAN))) >> (20 - MAN)) - (896 << MAN);
+    return u < (1 << MAN) ? 0 : min(u, 255 << MAN);
+  }
+  // to nearest, of a normal float that is known to `slack` units of its last place; -1 where that does not decide
   static __device__ __forceinline__ int rounded(float v, int slack) {
     const int b = __float_as_int(v), half = 1 << (22 - MAN), rest = (b & (2 * half - 1)) - half;
     return abs(rest) <= slack ? -1 : (b + half) >> (23 - MAN);
@@ -116,11 +125,10 @@ __device__ __forceinline__ void decode4(uint32_t cm, int em, uint32_t cr, int er
   }
 }
 
-__device__ __forceinline__ void encode4(const double m[4], const int rr[4], uint32_t& cm, int& em, uint32_t& cr, int& er) {
-  int rm[4], hm = 0, hr = 0;
+__device__ __forceinline__ void encode4(const double m[4], const int rm[4], const int rr[4], uint32_t& cm, int& em, uint32_t& cr, int& er) {
+  int hm = 0, hr = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    rm[k] = First::rounded(m[k]);
     hm = max(hm, rm[k]); hr = max(hr, rr[k]);
   }
   em = block_max(hm) >> 3; er = block_max(hr) >> 4;
@@ -133,12 +141,13 @@ __device__ __forceinline__ void encode4(const double m[4], const int rr[4], uint
   }
 }
 
-struct Rates { double beta1, beta2; float eps, scale; };
+struct Rates { double beta1, beta2; float eps, scale; uint64_t seed; };
 
-// the chunk of n elements (FULL: all of CHUNK) that begins at p's and g's `begin`; the state's pointers are the chunk's
-template <int BITS, bool FULL>
+// the chunk of n elements (FULL: all of CHUNK) that begins at p's and g's `begin`; the state's pointers are the chunk's, which
+// is the state's `at`-th element
+template <int BITS, bool RANDOM, bool FULL>
 __device__ __forceinline__ void adamw_chunk(int pt, void* pp, int gt, const void* gp, int64_t begin, int n, void* first_, void* second_,
-                                            uint8_t* first_e, uint8_t* second_e, const Rates& rate, const Scalars& sc) {
+                                            uint8_t* first_e, uint8_t* second_e, int64_t at, const Rates& rate, const Scalars& sc) {
   const int padded = (n + BLOCK - 1) / BLOCK * BLOCK;
   constexpr int TURNS = CHUNK / 1024;
   const float gs = rate.scale;
@@ -191,32 +200,50 @@ __device__ __forceinline__ void adamw_chunk(int pt, void* pp, int gt, const void
 #pragma clang fp contract(off)
       decode4(cm[u], em[u], cr[u], er[u], m, root);
       double dm[4];
-      int rr[4];
-      const float b2 = (float)rate.beta2, c2 = (float)(1.0 - rate.beta2);
-      bool unsure = false;
+      int r1[4], r2[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        dm[k] = (double)m[k] * rate.beta1 + (double)g[k] * (double)gs * (1.0 - rate.beta1);
-        m[k] = (float)dm[k];
-        const float gk = g[k] * gs, v = root[k] * root[k] * b2 + gk * c2 * gk, s = __builtin_amdgcn_sqrtf(v);
-        rr[k] = v == 0.f ? 0 : Root::rounded(s, 16);
-        const bool known = rr[k] >= 0 && (v == 0.f ? gk == 0.f && root[k] == 0.f : v > 1e-30f && v < 1e30f);
-        rr[k] = known ? rr[k] : -1;
-        unsure = unsure || !known;
-        if (known) root[k] = s;
-      }
-      if (unsure) {
+      for (int k = 0; k < 4; ++k) dm[k] = (double)m[k] * rate.beta1 + (double)g[k] * (double)gs * (1.0 - rate.beta1);
+      if constexpr (RANDOM) {
+        // Random rounding (Philox, counted by step and element): the moments' means go on where a step changes them by less than
+        // half a code, at b2 = 0.999 nearly always.  A word gives 16 bits to each of an element's codes.
+        const uint64_t index = (uint64_t)(at + i) / 4;
+        uint32_t c[4] = {(uint32_t)index, (uint32_t)(index >> 32), (uint32_t)sc.step, 1u};
+        philox4x32_10(c, (uint32_t)rate.seed, (uint32_t)(rate.seed >> 32));
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          if (rr[k] >= 0) continue;
           const double gk = (double)g[k] * (double)gs, r = root[k], s = sqrt(r * r * rate.beta2 + gk * (1.0 - rate.beta2) * gk);
-          rr[k] = Root::rounded(s);
+          r1[k] = First::rounded(dm[k], c[k] >> 16);
+          r2[k] = Root::rounded(s, c[k] & 0xFFFFu);
           root[k] = (float)s;
         }
+      } else {
+        const float b2 = (float)rate.beta2, c2 = (float)(1.0 - rate.beta2);
+        bool unsure = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          r1[k] = First::rounded(dm[k]);
+          const float gk = g[k] * gs, v = root[k] * root[k] * b2 + gk * c2 * gk, s = __builtin_amdgcn_sqrtf(v);
+          r2[k] = v == 0.f ? 0 : Root::rounded(s, 16);
+          const bool known = r2[k] >= 0 && (v == 0.f ? gk == 0.f && root[k] == 0.f : v > 1e-30f && v < 1e30f);
+          r2[k] = known ? r2[k] : -1;
+          unsure = unsure || !known;
+          if (known) root[k] = s;
+        }
+        if (unsure) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (r2[k] >= 0) continue;
+            const double gk = (double)g[k] * (double)gs, r = root[k], s = sqrt(r * r * rate.beta2 + gk * (1.0 - rate.beta2) * gk);
+            r2[k] = Root::rounded(s);
+            root[k] = (float)s;
+          }
+        }
       }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m[k] = (float)dm[k];
       uint32_t nm, nr;
       int fm, fr;
-      encode4(dm, rr, nm, fm, nr, fr);
+      encode4(dm, r1, r2, nm, fm, nr, fr);
       ((uint32_t*)first_)[i / 4] = nm;
       ((uint32_t*)second_)[i / 4] = nr;
       if ((threadIdx.x & 15) == 0) { first_e[i / BLOCK] = (uint8_t)fm; second_e[i / BLOCK] = (uint8_t)fr; }
@@ -227,23 +254,24 @@ __device__ __forceinline__ void adamw_chunk(int pt, void* pp, int gt, const void
   }
 }
 
-template <int BITS>
+template <int BITS, bool RANDOM>
 __global__ __launch_bounds__(256) void adamw_kernel(const rlgan_adamw_tensor_t* tensors, const int32_t* chunks, int64_t chunk0, int tensor0,
                                                     Grads grads, void* first, void* second, uint8_t* first_e, uint8_t* second_e,
-                                                    double beta1, double beta2, float eps, const float* grad_scale, const Scalars* scalars) {
+                                                    double beta1, double beta2, float eps, uint64_t seed, const float* grad_scale,
+                                                    const Scalars* scalars) {
   const Scalars sc = *scalars;
   if (sc.skip) return;
   const int ti = chunks[2 * (chunk0 + blockIdx.x)], ci = chunks[2 * (chunk0 + blockIdx.x) + 1];
   const rlgan_adamw_tensor_t T = tensors[ti];
   const void* gp = grads.p[ti - tensor0];
   const int gt = grads.type[ti - tensor0];
-  const Rates rate{beta1, beta2, eps, grad_scale ? *grad_scale : 1.f};
+  const Rates rate{beta1, beta2, eps, grad_scale ? *grad_scale : 1.f, seed};
   const int64_t begin = (int64_t)ci * CHUNK, at = T.offset + begin;
   constexpr int SIZE = BITS / 8;
   void* f = (char*)first + at * SIZE; void* s = (char*)second + at * SIZE;
   uint8_t* fe = BITS == 8 ? first_e + at / BLOCK : nullptr; uint8_t* se = BITS == 8 ? second_e + at / BLOCK : nullptr;
-  if (begin + CHUNK <= T.count) adamw_chunk<BITS, true>(T.type, T.param, gt, gp, begin, CHUNK, f, s, fe, se, rate, sc);
-  else adamw_chunk<BITS, false>(T.type, T.param, gt, gp, begin, (int)(T.count - begin), f, s, fe, se, rate, sc);
+  if (begin + CHUNK <= T.count) adamw_chunk<BITS, RANDOM, true>(T.type, T.param, gt, gp, begin, CHUNK, f, s, fe, se, at, rate, sc);
+  else adamw_chunk<BITS, RANDOM, false>(T.type, T.param, gt, gp, begin, (int)(T.count - begin), f, s, fe, se, at, rate, sc);
 }
 
 // 8-bit states as 32-bit numbers, and back
@@ -262,10 +290,11 @@ __global__ __launch_bounds__(256) void adamw_encode_kernel(const float4* m_in, c
   if (i >= n4) return;                              // n4 is a multiple of 16: whole blocks leave together
   const float4 a = m_in[i], b = v_in[i];
   const double m[4] = {a.x, a.y, a.z, a.w}, r[4] = {sqrt((double)b.x), sqrt((double)b.y), sqrt((double)b.z), sqrt((double)b.w)};
-  const int rr[4] = {Root::rounded(r[0]), Root::rounded(r[1]), Root::rounded(r[2]), Root::rounded(r[3])};
+  const int r1[4] = {First::rounded(m[0]), First::rounded(m[1]), First::rounded(m[2]), First::rounded(m[3])};
+  const int r2[4] = {Root::rounded(r[0]), Root::rounded(r[1]), Root::rounded(r[2]), Root::rounded(r[3])};
   uint32_t cm, cr;
   int em, er;
-  encode4(m, rr, cm, em, cr, er);
+  encode4(m, r1, r2, cm, em, cr, er);
   first[i] = cm; second[i] = cr;
   if ((threadIdx.x & 15) == 0) { first_e[i / 16] = (uint8_t)em; second_e[i / 16] = (uint8_t)er; }
 }
@@ -300,12 +329,13 @@ int rlgan_adamw_step(const rlgan_adamw_t* a, const void* const* grads, const uin
     for (int i = 0; i < n; ++i) { g.p[i] = grads[t0 + i]; g.type[i] = grad_types[t0 + i]; }
     const int64_t c0 = a->chunk_begin[t0], c1 = a->chunk_begin[t0 + n];
     if (c1 == c0) continue;
-    if (a->state_bits == 32)
-      hipLaunchKernelGGL(adamw_kernel<32>, dim3((unsigned)(c1 - c0)), dim3(256), 0, st, a->tensors, a->chunks, c0, t0, g, a->first, a->second,
-                         a->first_exp, a->second_exp, a->beta1, a->beta2, a->eps, grad_scale, (const Scalars*)a->scalars);
-    else
-      hipLaunchKernelGGL(adamw_kernel<8>, dim3((unsigned)(c1 - c0)), dim3(256), 0, st, a->tensors, a->chunks, c0, t0, g, a->first, a->second,
-                         a->first_exp, a->second_exp, a->beta1, a->beta2, a->eps, grad_scale, (const Scalars*)a->scalars);
+    const auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(c1 - c0)), dim3(256), 0, st, a->tensors, a->chunks, c0, t0, g, a->first, a->second, a->first_exp,
+                         a->second_exp, a->beta1, a->beta2, (float)a->eps, a->seed, grad_scale, (const Scalars*)a->scalars);
+    };
+    if (a->state_bits == 32) launch(adamw_kernel<32, false>);
+    else if (a->random) launch(adamw_kernel<8, true>);
+    else launch(adamw_kernel<8, false>);
   }
   return (int)hipGetLastError();
 }

@@ -210,6 +210,66 @@ def test_small_second_moments_do_not_explode(bits):
         assert (p - before).abs().max() <= 1e-2 * (4 if bits == 8 else 1.01)
 
 
+def test_random_rounding_of_one_step():
+    """Codes rounded at random against the same rounding of the oracle's moments with the oracle's Philox: a magnitude's 16 bits below
+    the code, plus 16 random bits, carry or do not."""
+    from oracle import philox
+    n, seed, t = 64 * 40, 0x123456789ABCDEF, 6
+    g = torch.Generator(device="cpu").manual_seed(9)
+    m0, v0 = torch.randn(n, generator=g).cuda(), torch.exp(torch.randn(n, generator=g)).cuda()
+    p, grad = torch.zeros(n, device="cuda"), torch.randn(n, generator=g).cuda()
+    opt = R.AdamW([p], state_bits=8, rounding="random", seed=seed, **HYPER)
+    opt.load_moments(m0, v0, t - 1)
+    m0, v0 = (_np(x) for x in opt.moments())
+    opt.step([grad])
+    m, v = (_np(x) for x in opt.moments())
+    em = m0 * BETAS[0] + _np(grad) * (1 - BETAS[0])
+    er = np.sqrt(v0 * BETAS[1] + _np(grad) * (1 - BETAS[1]) * _np(grad))
+    words = np.array([philox.philox4x32((i, 0, t, 1), (seed & 0xFFFFFFFF, seed >> 32)) for i in range(n // 4)]).reshape(-1)
+    for got, want, bits, man in ((np.abs(m), np.abs(em), words >> 16, 3), (np.sqrt(v), er, words & 0xFFFF, 4)):
+        high = want.astype(np.float64).view(np.int64) >> 32
+        high = (high + (bits << (4 - man))) >> (20 - man) << (20 - man)
+        np.testing.assert_array_equal(got, (high << 32).view(np.float64))   # all of these lie within the codes' 16 octaves
+    assert np.all(np.sign(m) == np.sign(em))
+
+
+def test_random_rounding_follows_the_mean():
+    """Second moments that decay by 1% a step, half a percent of the root, which is under half a code: to nearest they stay for
+    ever; at random their root's mean is the exact one.  A step's rounding has a deviation of at most half a code's 2^-4 of the
+    root, independent from step to step: over 300 steps some 2^-5 sqrt(300) = 0.55 of the mean for an element, 0.0034 for the mean
+    of 25600; 0.02 is six of those."""
+    n = 25600
+    for rounding in ("nearest", "random"):
+        p = torch.zeros(n, device="cuda")
+        opt = R.AdamW([p], state_bits=8, rounding=rounding, seed=3, **HYPER)
+        opt.load_moments(torch.zeros(n, device="cuda"), torch.full((n,), 4.0, device="cuda"), 10)
+        zero = torch.zeros(n, device="cuda")
+        for _ in range(300):
+            opt.step([zero])
+        root = opt.moments()[1].double().sqrt().mean().item()
+        if rounding == "nearest":
+            assert root == 2.0
+        else:
+            want = 2.0 * 0.99 ** 150
+            assert abs(root / want - 1) <= 0.02
+
+
+def test_random_rounding_repeats():
+    def run(seed, split):
+        params, grads = _make([1000, 77], ["fp32"], ["bf16"], 10)
+        opt = R.AdamW(params, state_bits=8, rounding="random", seed=seed, **HYPER)
+        for k in range(4):
+            opt.step(grads)
+            if k == split:                                       # the state handed on to another optimizer
+                other = R.AdamW(params, state_bits=8, rounding="random", seed=seed, **HYPER)
+                other.load_state_dict(opt.state_dict())
+                opt = other
+        return params + list(opt.moments())
+    a, b, c = run(5, None), run(5, 1), run(6, None)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert not torch.equal(a[2], c[2])
+
+
 def test_numbers_that_are_not_finite():
     """A NaN gradient spoils its own element (32 bits) or its block (8 bits) and nothing else."""
     for bits in (8, 32):
@@ -270,7 +330,8 @@ def test_refusals():
     bad = [lambda: R.AdamW([]), lambda: R.AdamW([p], state_bits=16), lambda: R.AdamW([p.cpu()]), lambda: R.AdamW([p.double()]),
            lambda: R.AdamW([p, p]), lambda: R.AdamW([p[:6], p[5:]]), lambda: R.AdamW([torch.zeros(4, 4, device="cuda").t()]),
            lambda: R.AdamW([p], betas=(1.0, 0.9)), lambda: R.AdamW([p], lr=-1.0), lambda: R.AdamW([p], eps=-1.0),
-           lambda: R.AdamW([p], weight_decay=float("nan"))]
+           lambda: R.AdamW([p], weight_decay=float("nan")),
+           lambda: R.AdamW([p], rounding="up"), lambda: R.AdamW([p], seed=-1)]
     opt = R.AdamW([p, torch.zeros(3, 4, device="cuda")])
     g = [torch.zeros(10, device="cuda"), torch.zeros(3, 4, device="cuda")]
     one = torch.ones(1, device="cuda")

@@ -20,11 +20,11 @@ def test_records_have_the_c_sizes(tmp_path):
             "rlgan_adamw_t": _lib.AdamWState}
     src = tmp_path / "sz.c"
     body = "".join(f'  printf("{n} %zu\\n", sizeof({n}));\n' for n in recs)
-    src.write_text(f'#include <stdio.h>\n#include "rlgan_amd.h"\nint main(void) {{\n{body}  printf("chunk %d\\n", RLGAN_ADAMW_CHUNK);\n  return 0;\n}}\n')
+    src.write_text(f'#include <stdio.h>\n#include "rlgan_amd.h"\nint main(void) {{\n{body}  printf("chunk %d\\nscalars %d\\n", RLGAN_ADAMW_CHUNK, RLGAN_ADAMW_SCALARS);\n  return 0;\n}}\n')
     exe = tmp_path / "sz"
     subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
     out = dict(line.split() for line in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines())
-    assert int(out.pop("chunk")) == _lib.ADAMW_CHUNK
+    assert int(out.pop("chunk")) == _lib.ADAMW_CHUNK and int(out.pop("scalars")) == 32
     for name, size in out.items():
         assert C.sizeof(recs[name]) == int(size), name
 
