@@ -653,7 +653,7 @@ enum { RLGAN_F32 = 0, RLGAN_BF16 = 1, RLGAN_F16 = 2 };
  * A sequence [b] ends at step lengths[b] (clamped to 0 .. length): outputs at and behind it are 0, the state stays.
  * rlgan_seq_t: strides in elements between batch rows and between steps; channels lie next to each other.  Rows may begin at
  * any element.  Outputs overlap no input (state_out may be state, dstate_in may be dstate).  The state is 32 bits whatever the
- * type; sums run in 32 bits. */
+ * type; sums run in 32 bits.  Fewer than 2^31 units (batch * width), at most 2^30 steps. */
 typedef struct { void* p; int64_t batch, time; } rlgan_seq_t;
 typedef struct {
   int32_t batch, length, width, type;      /* type: RLGAN_F32 / RLGAN_BF16 / RLGAN_F16 of z, x, h and their gradients */
@@ -683,7 +683,7 @@ int rlgan_gated_scan_backward(const rlgan_scan_t* s, rlgan_seq_t h, rlgan_seq_t 
  * logp, entropy, kl: the row's log p[a], H and e^d - d - 1 (0 without ref_logp).  A row is left out (zeros in every output, no
  * share in the loss, whatever its other numbers) when its action is negative, its weight 0, its action not legal or the action's
  * logit -inf.  Logits that are not legal are never used, whatever they hold.  An action >= vocab makes the row and the loss NaN.
- * dlogits may be logits. */
+ * dlogits may be logits; it overlaps no other input.  vocab at most 2^30, temperature from 1e-30 to 1e30. */
 typedef struct {
   int64_t rows;
   int32_t vocab, type;
@@ -692,7 +692,7 @@ typedef struct {
   const float *old_logp, *advantages;      /* device [rows] */
   const float* weights;                    /* device [rows], or NULL: 1 / rows each */
   const float* ref_logp;                   /* device [rows], or NULL: no KL term */
-  const uint8_t* legal; int64_t ld_legal;  /* device [rows][vocab] bytes, 0: not legal; or NULL */
+  const uint8_t* legal; int64_t ld_legal;  /* device [rows][vocab] bytes, 0: not legal (ld_legal 0: one row for all); or NULL */
   double clip_low, clip_high, kl_coef, entropy_coef, temperature;
   float *loss, *logp, *entropy, *kl;       /* device: [1], [rows] each */
   void* dlogits; int64_t ld_d;             /* device, or NULL */

@@ -560,8 +560,9 @@ int rlgan_policy_loss(const rlgan_policy_t* p, void* workspace, void* stream) {
     return RLGAN_E_ARG;
   if (p->rows <= 0 || p->vocab <= 0 || p->rows > INT32_MAX) return RLGAN_E_ARG;
   if (p->type < TYPE_F32 || p->type > TYPE_F16 || (p->action_bytes != 4 && p->action_bytes != 8)) return RLGAN_E_KIND;
-  if (p->ld < p->vocab || (p->dlogits && p->ld_d < p->vocab) || (p->legal && p->ld_legal < p->vocab)) return RLGAN_E_ALIGN;
-  if (!(p->temperature > 0)) return RLGAN_E_ARG;
+  if (p->vocab > 1 << 30) return RLGAN_E_DIMS;                          // columns are counted in 32 bits
+  if (p->ld < p->vocab || (p->dlogits && p->ld_d < p->vocab) || (p->legal && p->ld_legal && p->ld_legal < p->vocab)) return RLGAN_E_ALIGN;
+  if (!(p->temperature >= 1e-30 && p->temperature <= 1e30)) return RLGAN_E_ARG;
   Policy P{p->rows, p->vocab, p->ld, p->ld_legal, p->ld_d, p->actions, p->action_bytes == 8, p->old_logp, p->advantages, p->weights, p->ref_logp,
            p->legal, (float)(1.44269504088896340736 / p->temperature), 1.0 / p->temperature, p->clip_low, p->clip_high, p->kl_coef,
            p->entropy_coef, 1.0 / (double)p->rows, p->logp, p->entropy, p->kl};

@@ -451,7 +451,7 @@ inline int check_scan(const rlgan_scan_t* s) {
   if (!s || !s->z.p || !s->x.p) return RLGAN_E_ARG;
   if (s->batch <= 0 || s->length <= 0 || s->width <= 0) return RLGAN_E_ARG;
   if (s->type < TYPE_F32 || s->type > TYPE_F16) return RLGAN_E_KIND;
-  if ((int64_t)s->batch * s->width > (int64_t)1 << 31) return RLGAN_E_DIMS;
+  if ((int64_t)s->batch * s->width > INT32_MAX || s->length > 1 << 30) return RLGAN_E_DIMS;      // units and steps are counted in 32 bits
   return 0;
 }
 

@@ -32,7 +32,7 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logp: torch.Ten
 
     logits [rows, actions]: float32, bfloat16 or float16, any row stride.  actions: int32 or int64 [rows].  old_logp, advantages,
     weights, ref_logp: float32 [rows]; weights default to 1 / rows each (a mean over counted rows: weights = mask / mask.sum()).
-    legal: bool or uint8 [rows, actions], False for actions that cannot be chosen.  clip: one bound or (low, high).
+    legal: bool or uint8 [rows, actions], False for actions that cannot be chosen (one mask for all rows: mask.expand(rows, -1)).  clip: one bound or (low, high).
     out: tensor for the gradient, or the logits themselves to overwrite them.
 
     A row is left out, with zeros in every output, where its action is negative (padding), its weight is 0, or its action is not
@@ -41,13 +41,13 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logp: torch.Ten
     code = type_code(logits, "logits")
     need(logits.dim() == 2 and (logits.shape[1] <= 1 or logits.stride(1) == 1), "logits: [rows, actions] with a row's logits next to each other")
     rows, vocab = logits.shape
-    need(vocab > 0 and vocab < 1 << 31 and rows < 1 << 31, "logits: at least one action, fewer than 2^31 actions and rows")
+    need(0 < vocab <= 1 << 30 and rows < 1 << 31, "logits: 1 to 2^30 actions and fewer than 2^31 rows")
     on_device(actions, dev, "actions")
     need(actions.dtype in (torch.int32, torch.int64) and actions.shape == (rows,) and actions.is_contiguous(),
          "actions: contiguous int32 or int64 of shape [rows]")
     low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
     need(0 <= low <= 1 and high >= 0, "clip: bounds of at least 0, the lower one at most 1")
-    need(temperature > 0 and temperature < float("inf"), "temperature has to be positive")
+    need(1e-30 <= temperature <= 1e30, "temperature has to be positive (1e-30 to 1e30)")
     p_old, p_adv = vector(old_logp, (rows,), dev, "old_logp"), vector(advantages, (rows,), dev, "advantages")
     need(p_old is not None and p_adv is not None, "old_logp and advantages are wanted")
     p_w, p_ref = vector(weights, (rows,), dev, "weights"), vector(ref_logp, (rows,), dev, "ref_logp")

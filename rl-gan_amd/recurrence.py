@@ -37,7 +37,7 @@ def _scan(z, x, state, starts, lengths) -> Tuple[Scan, torch.device]:
     shape, dtype = z.shape, z.dtype
     need(len(shape) == 3, "z and x are [batch, time, width]")
     b, n, d = shape
-    need(b * d <= 1 << 31 and n < 1 << 31, "at most 2^31 units and steps")
+    need(b * d < 1 << 31 and n <= 1 << 30, "fewer than 2^31 units and at most 2^30 steps")
     st = None
     sb = ss = 0
     if starts is not None:
@@ -139,7 +139,7 @@ def gated_step(z: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *, starts:
     b, d = shape
     (zb, zc), (xb, xc) = z.stride(), x.stride()
     need(d <= 1 or zc == xc == 1, "z and x: channels have to lie next to each other")
-    need(b * d <= 1 << 31, "at most 2^31 units")
+    need(b * d < 1 << 31, "fewer than 2^31 units")
     need(state is not None, "state: a float32 tensor [batch, width] to advance")
     p_state = vector(state, shape, dev, "state")
     p_starts = starts_b = None
@@ -194,6 +194,7 @@ class GatedUnit:
 
     def backward(self, dh: torch.Tensor, dstate: Optional[torch.Tensor] = None, need_dx: bool = True):
         """(dx or None, dstate_in) of the latest `forward`; fills gates.grad."""
+        need(self._pass is not None, "backward without a forward pass")
         rows, both, h, state, starts, lengths = self._pass
         dboth = torch.empty_like(both)
         _, _, dstate_in = gated_scan_backward(dh, *self._split(both), h, state, starts=starts, lengths=lengths, dstate=dstate,

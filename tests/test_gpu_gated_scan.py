@@ -254,6 +254,23 @@ def test_captured_graphs_and_streams(n):
                 assert torch.equal(p, q), turn
 
 
+def test_rows_far_apart():
+    """Offsets that pass 32 bits: rows and steps of a buffer of more than 2^32 elements, forward and backward."""
+    b, n, d = 2, 70, 64
+    room = torch.empty((1 << 31) + (1 << 21), dtype=torch.bfloat16, device="cuda")
+    s = _inputs(b, n, d, "bf16", "plain", 15, starts=True)
+    want = R.gated_scan(s["z"], s["x"], s["state"], starts=s["starts"])
+    wantb = R.gated_scan_backward(s["dh"], s["z"], s["x"], want[0], s["state"], starts=s["starts"], dstate=s["dstate"])
+    for strides in ((1 << 31, 128, 1), (128, 31117312, 1)):       # batch rows, then steps, far apart
+        z, x = room.as_strided((b, n, d), strides), room.as_strided((b, n, d), strides, 64)
+        z.copy_(s["z"])
+        x.copy_(s["x"])
+        got = R.gated_scan(z, x, s["state"], starts=s["starts"])
+        gotb = R.gated_scan_backward(s["dh"], z, x, want[0], s["state"], starts=s["starts"], dstate=s["dstate"])
+        for p, q in zip(got + gotb, want + wantb):
+            assert torch.equal(p, q)
+
+
 def test_same_bits_every_time():
     s = _inputs(2, 7000, 48, "fp32", "plain", 13, True)
     first = R.gated_scan(s["z"], s["x"], s["state"], starts=s["starts"])

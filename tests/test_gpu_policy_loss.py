@@ -190,6 +190,28 @@ def test_masked_places_hold_anything(vocab, kind):
 
 
 @pytest.mark.parametrize("vocab", [6, 300, 9000, 60000])
+def test_one_mask_for_all_rows(vocab):
+    s = _inputs(9, vocab, "bf16", 17, legal=True)
+    mask = s["legal"][0].clone()
+    want = _call(dict(s, legal=mask.repeat(9, 1)))
+    got = _call(dict(s, legal=mask.expand(9, -1)))
+    for p, q in zip(got, want):
+        assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("vocab", [5, 3000])
+@pytest.mark.parametrize("temperature", [1e-3, 1e4])
+def test_far_temperatures(vocab, temperature):
+    """Nearly certain and nearly uniform: the oracle's numbers up to an exponent's rounding, which grows with x = dz / temperature."""
+    s = _inputs(6, vocab, "fp32", 18, ref=False)
+    got, ref = _call(s, temperature=temperature), _reference(s, temperature=temperature)
+    reach = float(s["logits"].abs().max()) * 2 / temperature
+    assert np.all(np.abs(_np(got.logp) - ref[1]) <= 4 * U * reach + 1e-5)
+    assert np.all(np.abs(_np(got.entropy) - ref[2]) <= 1e-4)
+    assert torch.isfinite(got.dlogits).all()
+
+
+@pytest.mark.parametrize("vocab", [6, 300, 9000, 60000])
 def test_rows_left_out(vocab):
     """Padding, weight 0, an action that is not allowed, no allowed action at all: zeros, whatever the row's other numbers are."""
     s = _inputs(8, vocab, "fp32", 8, legal=True)

@@ -43,7 +43,8 @@ def test_scan_refusals():
     assert fwd(_scan(batch=0)) == ARG and fwd(_scan(length=-1)) == ARG and fwd(_scan(width=0)) == ARG
     assert fwd(_scan(type=3)) == KIND and fwd(_scan(z=none)) == ARG and fwd(_scan(x=none)) == ARG
     assert fwd(_scan(), none) == ARG and fwd(_scan(), seq, None) == ARG
-    assert fwd(_scan(batch=1 << 30, width=4)) == DIMS
+    assert fwd(_scan(batch=1 << 30, width=4)) == DIMS and fwd(_scan(batch=1 << 16, width=1 << 15)) == DIMS
+    assert fwd(_scan(length=(1 << 30) + 1)) == DIMS
     bwd = lambda s, h=seq, dh=seq, dz=seq, dx=seq, ds=64: lib.rlgan_gated_scan_backward(C.byref(s), h, dh, None, dz, dx, ds, None, None)
     assert bwd(_scan(), h=none) == ARG and bwd(_scan(), dh=none) == ARG and bwd(_scan(), dz=none) == ARG
     assert bwd(_scan(), dx=none) == ARG and bwd(_scan(), ds=None) == ARG and bwd(_scan(type=-1)) == KIND
@@ -91,7 +92,8 @@ def test_policy_refusals():
     assert call(_policy(rows=0)) == ARG and call(_policy(rows=1 << 31)) == ARG and call(_policy(vocab=0)) == ARG
     assert call(_policy(type=3)) == KIND and call(_policy(action_bytes=2)) == KIND
     assert call(_policy(ld=4)) == ALIGN and call(_policy(dlogits=64, ld_d=4)) == ALIGN and call(_policy(legal=64, ld_legal=3)) == ALIGN
-    for t in (0.0, -1.0, float("nan")):
+    assert call(_policy(vocab=(1 << 30) + 1, ld=1 << 31)) == DIMS
+    for t in (0.0, -1.0, float("nan"), float("inf"), 1e-39):
         assert call(_policy(temperature=t)) == ARG
     n = C.c_int64()
     assert lib.rlgan_policy_loss_workspace(0, 5, 0, C.byref(n)) == ARG and lib.rlgan_policy_loss_workspace(3, 5, 9, C.byref(n)) == KIND
