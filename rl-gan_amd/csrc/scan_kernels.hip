@@ -425,26 +425,284 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_walk_bwd(Units u, Seq<cons
   }
 }
 
+// ---- the chained form -----------------------------------------------------------------------------------------
+// Few units and many steps, inputs read once: a workgroup holds a chunk of steps in registers, folds it to its map, hands the map
+// on through memory, looks back over the chunks before it as far as one whose state is already known, hands its own state on, and
+// runs its steps from registers.  A map or state is one 8-byte word (written and read as a whole, at device scope), and a word that
+// is not there yet is all ones: no other memory needs ordering.  Every wait ends: chunks are numbered by a ticket that a workgroup
+// draws when it runs; it waits for the maps of chunks with smaller tickets, whose workgroups run and hand those on without waiting
+// for anything, and at most for the state of one such chunk, which by the same argument from the first chunk on is handed on too.
+
+// Steps of a wave in a chunk, forward and backward.  More of them wait less for each other, fewer leave room for a second workgroup
+// a CU: 65536 steps of 512 units fp32 forward 124, 102, 102 us with 8, 12, 16; 16385 of 3000 bf16 backward 182, 174, 168 with 8, 10, 12.
+constexpr int CHAIN_FORWARD = 16, CHAIN_BACKWARD = 12;
+constexpr uint64_t NONE = ~0ull;
+struct Chain { int tiles, chunks; uint32_t* ticket; uint64_t* maps; uint64_t* states; };    // [chunk + 1][unit]; 0: what the call was handed
+
+__device__ __forceinline__ uint64_t word_of(Map m) {
+  const uint64_t w = (uint64_t)__float_as_uint(m.b) << 32 | __float_as_uint(m.a);
+  return w == NONE ? NONE >> 1 : w;                  // (a NaN either way)
+}
+__device__ __forceinline__ Map map_of(uint64_t w) { return {__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32))}; }
+__device__ __forceinline__ void hand_on(uint64_t* p, uint64_t w) { __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint64_t look_at(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// (the state handed in goes in front of the others: the call may overwrite it)
+__global__ __launch_bounds__(256) void scan_chain_clear_kernel(Chain ch, int64_t units, const float* handed) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (ch.chunks + 1) * units;
+  if (i < n) {
+    ch.maps[i] = NONE;
+    ch.states[i] = i < units ? word_of({DROP, handed ? handed[i] : 0.f}) : NONE;
+  }
+  if (i == 0) *ch.ticket = 0;
+}
+
+__device__ __forceinline__ Place draw(const Chain& ch, uint32_t* sh) {
+  if (threadIdx.x == 0) *sh = __hip_atomic_fetch_add(ch.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  const int t = __builtin_amdgcn_readfirstlane((int)*sh);
+  return {t % ch.tiles, t / ch.tiles};
+}
+
+constexpr int DEPTH = 8;                             // rounds of WAVES chunks that a workgroup looks back at most
+
+template <int VEC> struct ChunkShared {
+  Map own[WAVES][64 * VEC], before[DEPTH * WAVES][64 * VEC];
+  float state[64 * VEC];
+  uint32_t ticket;
+};
+
+// The state s in front of this workgroup's chunk, whose waves' maps are in sh.own (BACK: the last wave's applies first), and `after`
+// it.  Round by round each wave looks at one of the chunks before, nearest first, until every unit has a state or a map that lets
+// nothing through; the last round's furthest chunk is waited for until its state is known (it is, once the chunks before that one
+// are done, which wait for none of this).  The maps are then applied from the furthest on, as a walk through the chunks in order
+// would: the same bits whichever states were there already.
+template <int VEC, bool BACK>
+__device__ __forceinline__ void enter_chunk(const Lanes<VEC>& me, const Chain& ch, int chunk, int64_t units, ChunkShared<VEC>& sh, float s[VEC],
+                                            float after[VEC]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  Map total[VEC];
+  bool seen[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    total[k] = {1.f, 0.f};
+    seen[k] = false;
+  }
+  if (wave == 0) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) total[k] = compose(sh.own[BACK ? WAVES - 1 - w : w][lane * VEC + k], total[k]);
+      if (me.real) hand_on(ch.maps + (int64_t)(chunk + 1) * units + me.unit + k, word_of(total[k]));
+    }
+  }
+  int rounds = 0;
+  for (bool done = false; !done; ++rounds) {
+    const int p = chunk - 1 - rounds * WAVES - wave;         // -1: what the call was handed
+    const bool last = rounds == DEPTH - 1 && wave == WAVES - 1;
+    uint64_t w[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) w[k] = word_of({1.f, 0.f});
+    if (p >= -1) {
+      const int64_t at = (int64_t)(p + 1) * units + me.unit;
+      for (bool wait = true; wait;) {
+        uint64_t map[VEC];
+        wait = false;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) { w[k] = look_at(ch.states + at + k); map[k] = look_at(ch.maps + at + k); }
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          if (w[k] == NONE && !last) w[k] = map[k];
+          wait = wait || w[k] == NONE;
+        }
+        if (wait) __builtin_amdgcn_s_sleep(1);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sh.before[rounds * WAVES + wave][lane * VEC + k] = map_of(w[k]);
+    __syncthreads();
+    done = true;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+#pragma unroll
+      for (int v = 0; v < WAVES; ++v) seen[k] = seen[k] || __float_as_int(sh.before[rounds * WAVES + v][lane * VEC + k].a) < 0;
+      done = done && seen[k];
+    }
+    done = __all(done);                              // the same in every wave: all look at the same units
+  }
+  if (wave == 0) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) s[k] = 0.f;
+    for (int r = rounds - 1; r >= 0; --r) {
+#pragma unroll
+      for (int v = WAVES - 1; v >= 0; --v)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) s[k] = apply(sh.before[r * WAVES + v][lane * VEC + k], s[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      sh.state[lane * VEC + k] = s[k];
+      after[k] = apply(total[k], s[k]);
+      if (me.real) hand_on(ch.states + (int64_t)(chunk + 1) * units + me.unit + k, word_of({DROP, after[k]}));
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) s[k] = sh.state[lane * VEC + k];
+}
+
+template <typename T, int VEC, bool MASK>
+__global__ __launch_bounds__(WAVES * 64, 4) void scan_chain_fwd(Units u, Seq<const T> z, Seq<const T> x, Seq<T> h, float* state_out, Chain ch) {
+  constexpr int ST = CHAIN_FORWARD;
+  __shared__ ChunkShared<VEC> sh;
+  const Place at = draw(ch, &sh.ticket);
+  const int chunk = at.segment;
+  const Lanes<VEC> me(u, at.tile, MASK);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t0 = (chunk * WAVES + wave) * ST;
+  const T* zp = z.p + me.b * z.b + me.d; const T* xp = x.p + me.b * x.b + me.d; T* hp = h.p + me.b * h.b + me.d;
+  Words<T, VEC> zv[ST], xv[ST];
+  load_steps(zv, zp, z.t, t0, u.length);
+  load_steps(xv, xp, x.t, t0, u.length);
+  const uint32_t st = load_starts<ST>(MASK && u.starts ? u.starts + me.b * u.starts_b : nullptr, u.starts_t, t0, u.length);
+  Map m[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) m[k] = {1.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < ST; ++i) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      float f, take;
+      gate(zv[i].get(k), f, take);
+      fold_forward(m[k], f, take, xv[i].get(k), MASK && ((st >> i) & 1), t0 + i < me.len);
+    }
+    zv[i].pin();
+  }
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) sh.own[wave][lane * VEC + k] = m[k];
+  __syncthreads();
+  float s[VEC], after[VEC];
+  enter_chunk<VEC, false>(me, ch, chunk, (int64_t)u.batch * u.width, sh, s, after);
+#pragma unroll
+  for (int k = 0; k < VEC; ++k)
+    for (int w = 0; w < wave; ++w) s[k] = apply(sh.own[w][lane * VEC + k], s[k]);
+#pragma unroll
+  for (int i = 0; i < ST; ++i) {
+    if (t0 + i >= u.length) break;
+    Vec<T, VEC> hv;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const bool live = !MASK || t0 + i < me.len;
+      float f, take;
+      gate(zv[i].get(k), f, take);
+      const float p = MASK && ((st >> i) & 1) ? 0.f : s[k], v = p + take * (xv[i].get(k) - p);
+      s[k] = live ? v : s[k];
+      hv.set(k, live ? v : 0.f);
+    }
+    if (me.real) hv.store(hp + (t0 + i) * h.t);
+  }
+  if (chunk == ch.chunks - 1 && wave == 0 && me.real) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) state_out[me.unit + k] = after[k];
+  }
+}
+
+template <typename T, int VEC, bool MASK>
+__global__ __launch_bounds__(WAVES * 64, 4) void scan_chain_bwd(Units u, Seq<const T> dh, Seq<const T> z, Seq<const T> x, Seq<const T> h,
+                                                               Seq<T> dz, Seq<T> dx, float* dstate_in, Chain ch) {
+  constexpr int ST = CHAIN_BACKWARD;
+  __shared__ ChunkShared<VEC> sh;
+  const Place at = draw(ch, &sh.ticket);
+  const int chunk = at.segment;                      // counted from the end of the time axis
+  const Lanes<VEC> me(u, at.tile, MASK);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t0 = ((ch.chunks - 1 - chunk) * WAVES + wave) * ST;
+  Words<T, VEC> zv[ST], xv[ST], gv[ST], hv[ST];
+  load_steps(zv, z.p + me.b * z.b + me.d, z.t, t0, u.length);
+  load_steps(gv, dh.p + me.b * dh.b + me.d, dh.t, t0, u.length);
+  load_steps(xv, x.p + me.b * x.b + me.d, x.t, t0, u.length);
+  load_steps(hv, h.p + me.b * h.b + me.d, h.t, t0 - 1, u.length);
+  const uint32_t st = load_starts<ST>(MASK && u.starts ? u.starts + me.b * u.starts_b : nullptr, u.starts_t, t0, u.length);
+  Map m[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) m[k] = {1.f, 0.f};
+#pragma unroll
+  for (int i = ST - 1; i >= 0; --i) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      float f, take;
+      gate(zv[i].get(k), f, take);
+      fold_backward(m[k], f, gv[i].get(k), MASK && ((st >> i) & 1), t0 + i < me.len);
+    }
+    zv[i].pin();
+  }
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) sh.own[wave][lane * VEC + k] = m[k];
+  __syncthreads();
+  float c[VEC], after[VEC];
+  enter_chunk<VEC, true>(me, ch, chunk, (int64_t)u.batch * u.width, sh, c, after);
+#pragma unroll
+  for (int k = 0; k < VEC; ++k)
+    for (int w = WAVES - 1; w > wave; --w) c[k] = apply(sh.own[w][lane * VEC + k], c[k]);
+  T* ozp = dz.p + me.b * dz.b + me.d; T* oxp = dx.p + me.b * dx.b + me.d;
+#pragma unroll
+  for (int i = ST - 1; i >= 0; --i) {
+    if (t0 + i >= u.length) continue;
+    Vec<T, VEC> oz, ox;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const bool live = !MASK || t0 + i < me.len, start = MASK && ((st >> i) & 1);
+      const float before = t0 + i > 0 ? hv[i].get(k) : u.state ? u.state[me.unit + k] : 0.f, p = start ? 0.f : before;
+      float f, take;
+      gate(zv[i].get(k), f, take);
+      const float g = c[k] + gv[i].get(k), gt = g * take;
+      ox.set(k, live ? gt : 0.f);
+      oz.set(k, live ? gt * f * (p - xv[i].get(k)) : 0.f);
+      c[k] = live ? (start ? 0.f : f * g) : c[k];
+    }
+    if (me.real) { oz.store(ozp + (t0 + i) * dz.t); ox.store(oxp + (t0 + i) * dx.t); }
+  }
+  if (chunk == ch.chunks - 1 && wave == 0 && me.real) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) dstate_in[me.unit + k] = after[k];
+  }
+}
+
 // ---- which form -------------------------------------------------------------------------------------------------
 
-// Up to SERIAL steps one thread a unit is best (a single step is one read and one write); behind that the tiled form.
+// Up to SERIAL steps one thread a unit is best (a single step is one read and one write); behind that the tiled form, where there
+// are few units cut into segments or, beyond CACHE bytes, chained.
 constexpr int SERIAL = 8;
+constexpr int64_t CACHE = 256ll << 20;
 
-struct Plan { bool serial; int vec; Cut cut; };
+struct Plan { bool serial, chained; int vec, steps; Cut cut; };
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // A cut costs a second read of two tensors, idle CUs cost bandwidth.  Measured on an MI355X with 256, 512, 1024, 2048 workgroups
 // wanted: 65536 steps of 512 units forward fp32 161, 145, 149, 154 us, 16385 of 3000 backward bf16 257, 223, 231, 237; and with 256 or
 // more workgroups of units (1024 steps of 32768 units bf16: 46 us) a cut loses (70 us in two segments).
-inline Plan plan(int batch, int length, int width, int size, int vec) {
+// The chain reads everything once but has workgroups wait for each other.  What the 256 MB cache holds is cheap to read twice, the
+// rest is not: cut / chained 36 / 39 us for 100 MB (4096 steps of 4096 units bf16 forward), 61 / 77 for 246 MB (20000 of 1024
+// backward), 141 / 102 for 402 MB (65536 of 512 fp32 forward), 211 / 168 for 590 MB (16385 of 3000 bf16 backward), 213 / 150 for 737 MB
+// (4000 of 15360 fp32 forward).
+inline Plan plan(int batch, int length, int width, int size, int vec, bool backward) {
   constexpr int WANT = 512;
-  Plan p{length <= SERIAL, vec, {(int)cdiv((int64_t)batch * (width / vec), 64), 0, 0, false, nullptr}};
+  const int64_t units = (int64_t)batch * width, bytes = (backward ? 6 : 3) * size * units * length;
+  Plan p{length <= SERIAL, false, vec, backward ? CHAIN_BACKWARD : CHAIN_FORWARD, {(int)cdiv(units / vec, 64), 0, 0, false, nullptr}};
   const int64_t segments = p.cut.tiles >= WANT / 2 ? 1 : cdiv(WANT, p.cut.tiles), steps = cdiv(cdiv(length, segments), TILE) * TILE;
   p.cut.segment = (int)steps;
   p.cut.segments = (int)cdiv(length, steps);
   p.cut.runs = p.cut.segments == 1 && width * size % 128 != 0;
+  p.chained = !p.serial && p.cut.segments > 1 && bytes > CACHE;
   return p;
+}
+inline Chain chain_of(const Plan& p, int length, int64_t units, void* workspace) {
+  Chain c{p.cut.tiles, (int)cdiv(length, WAVES * p.steps), (uint32_t*)workspace, (uint64_t*)workspace + 2, nullptr};
+  c.states = c.maps + (c.chunks + 1) * units;
+  return c;
+}
+inline int64_t workspace_of(const Plan& p, int length, int64_t units) {
+  if (p.serial || p.cut.segments == 1) return 0;
+  return p.chained ? 16 + 16 * (cdiv(length, WAVES * p.steps) + 1) * units : (p.cut.segments + 1) * units * (int64_t)sizeof(Map);
 }
 
 inline int check_scan(const rlgan_scan_t* s) {
@@ -494,8 +752,7 @@ int rlgan_gated_scan_workspace(int batch, int length, int width, int type, int b
   int64_t most = 0;                              // one or two units a lane: the call decides by its tensors' alignment
   for (int vec = 1; vec <= 2; ++vec) {
     if (width % vec) break;
-    const Plan p = plan(batch, length, width, type == TYPE_F32 ? 4 : 2, vec);
-    if (!p.serial && p.cut.segments > 1) most = std::max(most, (int64_t)(p.cut.segments + 1) * batch * width * (int64_t)sizeof(Map));
+    most = std::max(most, workspace_of(plan(batch, length, width, type == TYPE_F32 ? 4 : 2, vec, backward != 0), length, (int64_t)batch * width));
   }
   *bytes = most;
   return 0;
@@ -506,7 +763,7 @@ int rlgan_gated_scan_forward(const rlgan_scan_t* s, rlgan_seq_t h, float* state_
   if (!h.p || !state_out) return RLGAN_E_ARG;
   const Units u = units(s);
   const bool mask = s->starts || s->lengths;
-  Plan p = plan(s->batch, s->length, s->width, s->type == TYPE_F32 ? 4 : 2, vec_of(s, {s->z, s->x, h}));
+  Plan p = plan(s->batch, s->length, s->width, s->type == TYPE_F32 ? 4 : 2, vec_of(s, {s->z, s->x, h}), false);
   p.cut.maps = (Map*)workspace;
   hipStream_t st = (hipStream_t)stream;
   if (p.serial) {
@@ -514,11 +771,19 @@ int rlgan_gated_scan_forward(const rlgan_scan_t* s, rlgan_seq_t h, float* state_
     RLGAN_SCAN_VARIANT(16, hipLaunchKernelGGL((scan_serial_fwd<T, VEC, MASK>), grid, dim3(256), 0, st, u, in<T>(s->z), in<T>(s->x), out<T>(h), state_out));
     return (int)hipGetLastError();
   }
-  if (p.cut.segments > 1) {
-    if (!workspace) return RLGAN_E_ARG;
-    RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_fold_kernel<T, VEC, MASK, false>), dim3(p.cut.tiles * (p.cut.segments - 1)), dim3(WAVES * 64), 0, st, u,
-                                          in<T>(s->z), in<T>(s->x), s->state, p.cut));
+  if (p.cut.segments > 1 && !workspace) return RLGAN_E_ARG;
+  if (p.chained) {
+    const int64_t n = (int64_t)s->batch * s->width;
+    const Chain ch = chain_of(p, s->length, n, workspace);
+    if ((int64_t)ch.tiles * ch.chunks > INT32_MAX) return RLGAN_E_DIMS;
+    hipLaunchKernelGGL(scan_chain_clear_kernel, dim3((unsigned)cdiv((ch.chunks + 1) * n, 256)), dim3(256), 0, st, ch, n, s->state);
+    RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_chain_fwd<T, VEC, MASK>), dim3(ch.tiles * ch.chunks), dim3(WAVES * 64), 0, st, u, in<T>(s->z),
+                                             in<T>(s->x), out<T>(h), state_out, ch));
+    return (int)hipGetLastError();
   }
+  if (p.cut.segments > 1)
+    RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_fold_kernel<T, VEC, MASK, false>), dim3(p.cut.tiles * (p.cut.segments - 1)), dim3(WAVES * 64), 0,
+                                             st, u, in<T>(s->z), in<T>(s->x), s->state, p.cut));
   RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_walk_fwd<T, VEC, MASK>), dim3(p.cut.tiles * p.cut.segments), dim3(WAVES * 64), 0, st, u, in<T>(s->z),
                                         in<T>(s->x), out<T>(h), state_out, p.cut));
   return (int)hipGetLastError();
@@ -537,7 +802,7 @@ int rlgan_gated_scan_backward(const rlgan_scan_t* s, rlgan_seq_t h, rlgan_seq_t 
   if (!h.p || !dh.p || !dz.p || !dx.p || !dstate_in) return RLGAN_E_ARG;
   const Units u = units(s);
   const bool mask = s->starts || s->lengths;
-  Plan p = plan(s->batch, s->length, s->width, s->type == TYPE_F32 ? 4 : 2, vec_of(s, {s->z, s->x, h, dh, dz, dx}));
+  Plan p = plan(s->batch, s->length, s->width, s->type == TYPE_F32 ? 4 : 2, vec_of(s, {s->z, s->x, h, dh, dz, dx}), true);
   p.cut.maps = (Map*)workspace;
   hipStream_t st = (hipStream_t)stream;
   if (p.serial) {
@@ -546,11 +811,19 @@ int rlgan_gated_scan_backward(const rlgan_scan_t* s, rlgan_seq_t h, rlgan_seq_t 
                                           dstate, out<T>(dz), out<T>(dx), dstate_in));
     return (int)hipGetLastError();
   }
-  if (p.cut.segments > 1) {
-    if (!workspace) return RLGAN_E_ARG;
-    RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_fold_kernel<T, VEC, MASK, true>), dim3(p.cut.tiles * (p.cut.segments - 1)), dim3(WAVES * 64), 0, st, u,
-                                          in<T>(s->z), in<T>(dh), dstate, p.cut));
+  if (p.cut.segments > 1 && !workspace) return RLGAN_E_ARG;
+  if (p.chained) {
+    const int64_t n = (int64_t)s->batch * s->width;
+    const Chain ch = chain_of(p, s->length, n, workspace);
+    if ((int64_t)ch.tiles * ch.chunks > INT32_MAX) return RLGAN_E_DIMS;
+    hipLaunchKernelGGL(scan_chain_clear_kernel, dim3((unsigned)cdiv((ch.chunks + 1) * n, 256)), dim3(256), 0, st, ch, n, dstate);
+    RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_chain_bwd<T, VEC, MASK>), dim3(ch.tiles * ch.chunks), dim3(WAVES * 64), 0, st, u, in<T>(dh),
+                                             in<T>(s->z), in<T>(s->x), in<T>(h), out<T>(dz), out<T>(dx), dstate_in, ch));
+    return (int)hipGetLastError();
   }
+  if (p.cut.segments > 1)
+    RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_fold_kernel<T, VEC, MASK, true>), dim3(p.cut.tiles * (p.cut.segments - 1)), dim3(WAVES * 64), 0,
+                                             st, u, in<T>(s->z), in<T>(dh), dstate, p.cut));
   RLGAN_SCAN_VARIANT(4, hipLaunchKernelGGL((scan_walk_bwd<T, VEC, MASK>), dim3(p.cut.tiles * p.cut.segments), dim3(WAVES * 64), 0, st, u, in<T>(dh),
                                         in<T>(s->z), in<T>(s->x), in<T>(h), dstate, out<T>(dz), out<T>(dx), dstate_in, p.cut));
   return (int)hipGetLastError();

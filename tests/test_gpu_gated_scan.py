@@ -117,6 +117,13 @@ def test_long_sequences(b, n, d, kind, masked):
     _check(_inputs(b, n, d, kind, "plain", 3, masked, masked, reach=3.0), kind)
 
 
+@pytest.mark.parametrize("b,n,d,kind,masked", [(1, 11001, 2048, "fp32", False), (3, 7000, 1111, "fp32", True), (2, 12100, 2000, "bf16", True)])
+def test_long_and_large(b, n, d, kind, masked):
+    """Few units, many steps and more than the caches hold: workgroups hand maps and states on along the time axis.  (The widths are
+    large for the oracle's sake, which walks the steps one by one.)"""
+    _check(_inputs(b, n, d, kind, "plain", 16, masked, masked, reach=3.0), kind)
+
+
 def test_many_units():
     _check(_inputs(700, 12, 300, "bf16", "plain", 4, True, True), "bf16")
 
@@ -135,10 +142,10 @@ def test_extreme_gates():
         assert (h[0, 8].float() - h[0, 7].float()).abs().max() <= (2 * (13 * 40 + 32) * U + torch.finfo(t).eps) * top
 
 
-@pytest.mark.parametrize("n", [40, 3000])
-def test_nothing_passes_a_start_or_an_end(n):
+@pytest.mark.parametrize("n,d", [(40, 20), (3000, 20), (40000, 200)])
+def test_nothing_passes_a_start_or_an_end(n, d):
     """NaN in the state, in an episode before, and behind a sequence's end reaches neither outputs nor gradients."""
-    b, d = 3, 20
+    b = 3
     s = _inputs(b, n, d, "fp32", "plain", 6, reach=3.0)
     s["starts"] = torch.zeros(b, n, dtype=torch.bool, device="cuda")
     s["starts"][0, 0] = True
@@ -162,7 +169,7 @@ def test_nothing_passes_a_start_or_an_end(n):
     assert (dz[2, n // 3:] == 0).all() and (dx[2, n // 3:] == 0).all()
 
 
-@pytest.mark.parametrize("n", [5, 4000])
+@pytest.mark.parametrize("n", [5, 4000, 1000000])
 def test_absent_state_and_gradient_are_zeros(n):
     s = _inputs(2, n, 12, "fp32", "plain", 7)
     zero = torch.zeros_like(s["state"])
@@ -222,7 +229,7 @@ def test_outputs_in_the_callers_buffers():
         assert torch.equal(a[0], b[0]) and torch.equal(both[..., :24], a[0]) and torch.equal(both[..., 24:], a[1])
 
 
-@pytest.mark.parametrize("n", [9, 5000])
+@pytest.mark.parametrize("n", [9, 5000, 360000])
 def test_captured_graphs_and_streams(n):
     """Two captured graphs and eager calls in turn, on a stream of their own: every replay gives the eager result."""
     a, b = _inputs(2, n, 32, "fp32", "plain", 11, True, True), _inputs(3, n, 20, "bf16", "plain", 12)
@@ -254,6 +261,22 @@ def test_captured_graphs_and_streams(n):
                 assert torch.equal(p, q), turn
 
 
+def test_two_streams_at_once():
+    """Long scans on two streams at the same time: workgroups of both wait and go on among each other."""
+    a, b = _inputs(2, 250000, 48, "fp32", "plain", 17), _inputs(1, 400000, 64, "fp32", "plain", 18)
+    want = [R.gated_scan(s["z"], s["x"], s["state"]) for s in (a, b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for turn in range(4):
+        for s, stream in zip((a, b), streams):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                got.append(R.gated_scan(s["z"], s["x"], s["state"]))
+    torch.cuda.synchronize()
+    for i, (h, last) in enumerate(got):
+        assert torch.equal(h, want[i % 2][0]) and torch.equal(last, want[i % 2][1])
+
+
 def test_rows_far_apart():
     """Offsets that pass 32 bits: rows and steps of a buffer of more than 2^32 elements, forward and backward."""
     b, n, d = 2, 70, 64
@@ -271,12 +294,14 @@ def test_rows_far_apart():
             assert torch.equal(p, q)
 
 
-def test_same_bits_every_time():
-    s = _inputs(2, 7000, 48, "fp32", "plain", 13, True)
-    first = R.gated_scan(s["z"], s["x"], s["state"], starts=s["starts"])
-    for _ in range(3):
-        again = R.gated_scan(s["z"], s["x"], s["state"], starts=s["starts"])
-        assert all(torch.equal(p, q) for p, q in zip(first, again))
+@pytest.mark.parametrize("n", [7000, 250000])
+def test_same_bits_every_time(n):
+    """Whatever order the workgroups of a long sequence come in."""
+    s = _inputs(2, n, 48, "fp32", "plain", 13, reach=4.0)
+    call = lambda h: R.gated_scan(s["z"], s["x"], s["state"]) + R.gated_scan_backward(s["dh"], s["z"], s["x"], h, s["state"], dstate=s["dstate"])
+    first = call(R.gated_scan(s["z"], s["x"], s["state"])[0])
+    for _ in range(5):
+        assert all(torch.equal(p, q) for p, q in zip(first, call(first[0])))
 
 
 def test_gated_unit_against_autograd():
