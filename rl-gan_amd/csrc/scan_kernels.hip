@@ -32,8 +32,8 @@ struct Units {
 template <typename T> struct Seq { T* p; int64_t b, t; };
 
 // ---- the serial form ----------------------------------------------------------------------------------------------
-// One thread a unit (VEC units), all steps in a row: for a single step, which is one read and one write, and up to SERIAL.  Bound by
-// memory, and by the launch where there is little: 4096 x 256 units fp32, one step, 5.2 us on an MI355X (4.0 TB/s from the caches).
+// One thread a unit (VEC units), all steps in a row: for a single step, which is one read and one write, and for few.  Bound by memory,
+// and by the launch where there is little: 4096 x 256 units fp32, one step, 5.2 us on an MI355X (4.0 TB/s from the caches).
 template <typename T, int VEC, bool MASK>
 __global__ __launch_bounds__(256) void scan_serial_fwd(Units u, Seq<const T> z, Seq<const T> x, Seq<T> h, float* state_out) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -673,9 +673,12 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_chain_bwd(Units u, Seq<con
 
 // ---- which form -------------------------------------------------------------------------------------------------
 
-// Up to SERIAL steps one thread a unit is best (a single step is one read and one write); behind that the tiled form, where there
-// are few units cut into segments or, beyond CACHE bytes, chained.
-constexpr int SERIAL = 8;
+// One thread a unit for up to 8 steps, and for up to 32 where the units fill the chip by themselves: a workgroup of the tiled form costs
+// the same whatever part of its 64 steps there is.  Measured, serial / tiled forward and backward, fp32: 16 steps of 32768 units 6.2 /
+// 5.1 and 7.7 / 5.4 us, of 131072 units 7.8 / 12.6 and 11.9 / 13.7, of 524288 17.9 / 40.5 and 32.9 / 43.3; 32 of 524288 32.4 / 43.7 and 78.4 /
+// 80.5, 48 of 524288 53 / 59 and 122 / 118; bf16: 16 of 262144 10.0 / 17.4 and 18.4 / 18.5.  Else the tiled form, where there are few
+// units cut into segments or, beyond CACHE bytes, chained.
+inline bool is_serial(int64_t units, int length, int size) { return length <= 8 || (length <= 32 && (int64_t)length * 32768 <= units * size); }
 constexpr int64_t CACHE = 256ll << 20;
 
 struct Plan { bool serial, chained; int vec, steps; Cut cut; };
@@ -692,7 +695,7 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline Plan plan(int batch, int length, int width, int size, int vec, bool backward) {
   constexpr int WANT = 512;
   const int64_t units = (int64_t)batch * width, bytes = (backward ? 6 : 3) * size * units * length;
-  Plan p{length <= SERIAL, false, vec, backward ? CHAIN_BACKWARD : CHAIN_FORWARD, {(int)cdiv(units / vec, 64), 0, 0, false, nullptr}};
+  Plan p{is_serial(units, length, size), false, vec, backward ? CHAIN_BACKWARD : CHAIN_FORWARD, {(int)cdiv(units / vec, 64), 0, 0, false, nullptr}};
   const int64_t segments = p.cut.tiles >= WANT / 2 ? 1 : cdiv(WANT, p.cut.tiles), steps = cdiv(cdiv(length, segments), TILE) * TILE;
   p.cut.segment = (int)steps;
   p.cut.segments = (int)cdiv(length, steps);
@@ -729,7 +732,7 @@ inline Units units(const rlgan_scan_t* s) {
 // form; 4 bytes in the tiled one, where 8 and 16 cost more in registers than wide loads give (1024 steps of 32768 units forward
 // bf16: 46 us with 2 units, 76 with 4, 50 with 1; backward of 25800 units fp32: 40 with 1, 48 with 2).
 inline int vec_of(const rlgan_scan_t* s, std::initializer_list<rlgan_seq_t> seqs) {
-  const int size = s->type == TYPE_F32 ? 4 : 2, vec = (s->length <= SERIAL ? 16 : 4) / size;
+  const int size = s->type == TYPE_F32 ? 4 : 2, vec = (is_serial((int64_t)s->batch * s->width, s->length, size) ? 16 : 4) / size;
   bool ok = s->width % vec == 0;
   for (const rlgan_seq_t& q : seqs) ok = ok && (uintptr_t)q.p % (vec * size) == 0 && q.batch % vec == 0 && q.time % vec == 0;
   return ok ? vec : 1;

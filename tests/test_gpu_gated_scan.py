@@ -124,8 +124,9 @@ def test_long_and_large(b, n, d, kind, masked):
     _check(_inputs(b, n, d, kind, "plain", 16, masked, masked, reach=3.0), kind)
 
 
-def test_many_units():
-    _check(_inputs(700, 12, 300, "bf16", "plain", 4, True, True), "bf16")
+@pytest.mark.parametrize("b,n,d,kind", [(700, 12, 300, "bf16"), (1024, 9, 301, "fp32"), (1500, 31, 256, "fp16"), (1024, 33, 256, "fp32")])
+def test_many_units(b, n, d, kind):
+    _check(_inputs(b, n, d, kind, "fused", 4, True, True), kind)
 
 
 def test_extreme_gates():
