@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "librlgan_amd.so")
@@ -157,6 +158,10 @@ class Policy(C.Structure):
                 ("dlogits", _fp), ("ld_d", C.c_int64)]
 
 
+# rlgan_scan_t and rlgan_policy_t as bytes, for calls whose host time counts: packing takes a quarter of filling a ctypes record
+PACK_SCAN = struct.Struct("@4iP2qP2q2P2qP").pack
+PACK_POLICY = struct.Struct("@q2iPqPi5Pq5d5Pq").pack
+
 ADAMW_CHUNK, ADAMW_BLOCK = 2048, 64                              # RLGAN_ADAMW_CHUNK; elements that share an exponent
 
 
@@ -268,11 +273,11 @@ PROTOTYPES = {
     "rlgan_dense_backward_weights": [_vp, _i, _vp, _i, _vp, _i, _i, _i, _vp, _i, _vp],
     "rlgan_dense_backward_kernel": [_vp, _i, _vp, _i, _vp, _i, _i, _i, _vp, _i, _vp],
     "rlgan_gated_scan_workspace": [_i, _i, _i, _i, _i, C.POINTER(C.c_int64)],
-    "rlgan_gated_scan_forward": [C.POINTER(Scan), SeqRef, _vp, _vp, _vp],
-    "rlgan_gated_scan_backward": [C.POINTER(Scan), SeqRef, SeqRef, _vp, SeqRef, SeqRef, _vp, _vp, _vp],
+    "rlgan_gated_scan_forward": [_vp, SeqRef, _vp, _vp, _vp],
+    "rlgan_gated_scan_backward": [_vp, SeqRef, SeqRef, _vp, SeqRef, SeqRef, _vp, _vp, _vp],
     "rlgan_gated_step": [_i, _i, _i, _vp, C.c_int64, _vp, C.c_int64, _vp, _vp, C.c_int64, _vp, _vp],
     "rlgan_policy_loss_workspace": [C.c_int64, _i, _i, C.POINTER(C.c_int64)],
-    "rlgan_policy_loss": [C.POINTER(Policy), _vp, _vp],
+    "rlgan_policy_loss": [_vp, _vp, _vp],
     "rlgan_adamw_step": [C.POINTER(AdamWState), _vp, _vp, _vp, _vp, _vp],
     "rlgan_adamw_decode": [_vp, _vp, _vp, _vp, C.c_int64, _vp, _vp, _vp],
     "rlgan_adamw_encode": [_vp, _vp, C.c_int64, _vp, _vp, _vp, _vp, _vp],

@@ -9,7 +9,7 @@ from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
-from ._lib import Policy, check, lib
+from ._lib import PACK_POLICY, check, lib
 from .tensors import apart, first_device, guard, need, on_device, own_elements, stream_of, type_code, vector
 
 
@@ -51,7 +51,7 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logp: torch.Ten
     p_old, p_adv = vector(old_logp, (rows,), dev, "old_logp"), vector(advantages, (rows,), dev, "advantages")
     need(p_old is not None and p_adv is not None, "old_logp and advantages are wanted")
     p_w, p_ref = vector(weights, (rows,), dev, "weights"), vector(ref_logp, (rows,), dev, "ref_logp")
-    p_legal, ld_legal = None, 0
+    p_legal = ld_legal = 0
     if legal is not None:
         on_device(legal, dev, "legal")
         need(legal.dtype in (torch.bool, torch.uint8) and legal.shape == logits.shape and (vocab == 1 or legal.stride(1) == 1),
@@ -86,10 +86,10 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logp: torch.Ten
         loss = torch.empty((), dtype=torch.float32, device=dev)
         base = room.data_ptr()
         out_at = base + 4 * words
-        args = Policy(rows, vocab, code, logits.data_ptr(), ld, actions.data_ptr(), actions.element_size(), p_old, p_adv, p_w, p_ref, p_legal,
-                      ld_legal, low, high, kl_coef, entropy_coef, temperature, loss.data_ptr(), out_at, out_at + 4 * rows, out_at + 8 * rows,
-                      None if d is None else d.data_ptr(), 0 if d is None else _row_stride(d, vocab))
-        check(lib.rlgan_policy_loss(C.byref(args), base, stream_of(dev)), "rlgan_policy_loss")
+        record = PACK_POLICY(rows, vocab, code, logits.data_ptr(), ld, actions.data_ptr(), actions.element_size(), p_old, p_adv, p_w or 0,
+                             p_ref or 0, p_legal, ld_legal, low, high, kl_coef, entropy_coef, temperature, loss.data_ptr(), out_at,
+                             out_at + 4 * rows, out_at + 8 * rows, *((0, 0) if d is None else (d.data_ptr(), _row_stride(d, vocab))))
+        check(lib.rlgan_policy_loss(record, base, stream_of(dev)), "rlgan_policy_loss")
     _, logp, entropy, kl = room.split([words, rows, rows, rows])
     return PolicyLoss(loss, logp, entropy, kl, d)
 

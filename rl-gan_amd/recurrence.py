@@ -11,41 +11,49 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import numpy as np
 import torch
 
-from ._lib import Scan, SeqRef, check, lib
+from ._lib import PACK_SCAN, SeqRef, check, lib
 from .conv import DenseLayer
 from .tensors import apart, byte_range, first_device, guard, need, on_device, stream_of, type_code, vector, workspace
 
 
-def _seq(t: torch.Tensor, shape, dtype, dev: torch.device, name: str) -> SeqRef:
+def _seq(t: torch.Tensor, shape, dtype, dev: torch.device, name: str):
+    """(pointer, batch stride, time stride) of a sequence tensor."""
     if t.get_device() != dev.index or t.dtype != dtype or t.shape != shape:
         on_device(t, dev, name)
         raise ValueError(f"{name}: {dtype} of shape {tuple(shape)} is wanted, got {t.dtype} {tuple(t.shape)}")
     b, n, c = t.stride()
     if c != 1 and shape[2] > 1:
         raise ValueError(f"{name}: channels have to lie next to each other (strides {t.stride()})")
-    return SeqRef(t.data_ptr(), b, n)
+    return t.data_ptr(), b, n
 
 
-def _scan(z, x, state, starts, lengths) -> Tuple[Scan, torch.device]:
+class _Call(NamedTuple):
+    record: bytes                             # rlgan_scan_t
+    dev: torch.device
+    shape: torch.Size
+    code: int
+
+
+def _scan(z, x, state, starts, lengths) -> _Call:
     dev = first_device(z, "z")
     code = type_code(z, "z")
     shape, dtype = z.shape, z.dtype
     need(len(shape) == 3, "z and x are [batch, time, width]")
     b, n, d = shape
     need(b * d < 1 << 31 and n <= 1 << 30, "fewer than 2^31 units and at most 2^30 steps")
-    st = None
-    sb = ss = 0
+    st = sb = ss = 0
     if starts is not None:
         on_device(starts, dev, "starts")
         need(starts.dtype in (torch.bool, torch.uint8) and starts.shape == shape[:2], "starts: bool or uint8 of shape [batch, time]")
         st, (sb, ss) = starts.data_ptr(), starts.stride()
-    return Scan(b, n, d, code, _seq(z, shape, dtype, dev, "z"), _seq(x, shape, dtype, dev, "x"), vector(state, (b, d), dev, "state"), st,
-                sb, ss, vector(lengths, (b,), dev, "lengths", torch.int32)), dev
+    record = PACK_SCAN(b, n, d, code, *_seq(z, shape, dtype, dev, "z"), *_seq(x, shape, dtype, dev, "x"), vector(state, (b, d), dev, "state") or 0,
+                       st, sb, ss, vector(lengths, (b,), dev, "lengths", torch.int32) or 0)
+    return _Call(record, dev, shape, code)
 
 
 def _output(out, like, others, name):
@@ -62,8 +70,9 @@ def _workspace_bytes(batch: int, length: int, width: int, code: int, backward: i
     return size.value
 
 
-def _workspace(s: Scan, backward: int, dev) -> Optional[torch.Tensor]:
-    return workspace(_workspace_bytes(s.batch, s.length, s.width, s.type, backward), dev)
+def _workspace(call: _Call, backward: int) -> Optional[torch.Tensor]:
+    b, n, d = call.shape
+    return workspace(_workspace_bytes(b, n, d, call.code, backward), call.dev)
 
 
 def gated_scan(z: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tensor] = None, *, starts: Optional[torch.Tensor] = None,
@@ -73,15 +82,16 @@ def gated_scan(z: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tensor] =
     state: what the sequences continue from (zeros if None).  starts: bool [batch, time], True where an episode begins: nothing
     from before reaches that step.  lengths: int32 [batch], steps of each sequence (clamped to 0 .. time); h is 0 at and behind
     a sequence's end, whatever z and x hold there, and the state is the one at its end."""
-    s, dev = _scan(z, x, state, starts, lengths)
+    call = _scan(z, x, state, starts, lengths)
+    dev, (b, _, d) = call.dev, call.shape
     h = _output(out, z, (z, x, state, starts, lengths), "out")
-    ref = _seq(h, z.shape, z.dtype, dev, "out")
-    if z.numel() == 0:
-        return h, torch.zeros((s.batch, s.width), dtype=torch.float32, device=dev) if state is None else state.clone()
+    ref = SeqRef(*_seq(h, z.shape, z.dtype, dev, "out"))
+    if h.numel() == 0:
+        return h, torch.zeros((b, d), dtype=torch.float32, device=dev) if state is None else state.clone()
     with guard(dev):
-        last = torch.empty((s.batch, s.width), dtype=torch.float32, device=dev)
-        ws = _workspace(s, 0, dev)
-        check(lib.rlgan_gated_scan_forward(C.byref(s), ref, last.data_ptr(), None if ws is None else ws.data_ptr(), stream_of(dev)),
+        last = torch.empty((b, d), dtype=torch.float32, device=dev)
+        ws = _workspace(call, 0)
+        check(lib.rlgan_gated_scan_forward(call.record, ref, last.data_ptr(), None if ws is None else ws.data_ptr(), stream_of(dev)),
               "rlgan_gated_scan_forward")
     return h, last
 
@@ -95,23 +105,25 @@ def gated_scan_backward(dh: torch.Tensor, z: torch.Tensor, x: torch.Tensor, h: t
     h: what the forward pass returned, in its type (for 16 bits it carries that type's rounding into dz: the alternative is a
     second forward scan).  out: tensors for dz and dx, which may be the halves of one buffer.  At and behind a sequence's end dz
     and dx are 0, whatever dh holds there."""
-    s, dev = _scan(z, x, state, starts, lengths)
-    rh, rdh = _seq(h, z.shape, z.dtype, dev, "h"), _seq(dh, z.shape, z.dtype, dev, "dh")
-    dst = vector(dstate, (s.batch, s.width), dev, "dstate")
+    call = _scan(z, x, state, starts, lengths)
+    dev, shape, dtype = call.dev, call.shape, z.dtype
+    b, _, d = shape
+    rh, rdh = _seq(h, shape, dtype, dev, "h"), _seq(dh, shape, dtype, dev, "dh")
+    dst = vector(dstate, (b, d), dev, "dstate")
     inputs = (z, x, h, dh, state, starts, lengths, dstate)
     if out is not None:
         need(len(out) == 2, "out: (dz, dx)")
         _halves_apart(*out)
     dz = _output(None if out is None else out[0], z, inputs, "out[0]")
     dx = _output(None if out is None else out[1], z, inputs, "out[1]")
-    rdz, rdx = _seq(dz, z.shape, z.dtype, dev, "out[0]"), _seq(dx, z.shape, z.dtype, dev, "out[1]")
-    if z.numel() == 0:
-        return dz, dx, torch.zeros((s.batch, s.width), dtype=torch.float32, device=dev) if dstate is None else dstate.clone()
+    rdz, rdx = _seq(dz, shape, dtype, dev, "out[0]"), _seq(dx, shape, dtype, dev, "out[1]")
+    if dz.numel() == 0:
+        return dz, dx, torch.zeros((b, d), dtype=torch.float32, device=dev) if dstate is None else dstate.clone()
     with guard(dev):
-        first = torch.empty((s.batch, s.width), dtype=torch.float32, device=dev)
-        ws = _workspace(s, 1, dev)
-        check(lib.rlgan_gated_scan_backward(C.byref(s), rh, rdh, dst, rdz, rdx, first.data_ptr(), None if ws is None else ws.data_ptr(),
-                                            stream_of(dev)), "rlgan_gated_scan_backward")
+        first = torch.empty((b, d), dtype=torch.float32, device=dev)
+        ws = _workspace(call, 1)
+        check(lib.rlgan_gated_scan_backward(call.record, SeqRef(*rh), SeqRef(*rdh), dst, SeqRef(*rdz), SeqRef(*rdx), first.data_ptr(),
+                                            None if ws is None else ws.data_ptr(), stream_of(dev)), "rlgan_gated_scan_backward")
     return dz, dx, first
 
 

@@ -29,6 +29,19 @@ def test_records_have_the_c_sizes(tmp_path):
         assert C.sizeof(recs[name]) == int(size), name
 
 
+def test_packed_records_are_the_records():
+    seq = (11, 12, 13)
+    s = _lib.Scan(1, 2, 3, 2, _lib.SeqRef(*seq), _lib.SeqRef(21, 22, 23), 31, 32, 33, 34, 35)
+    assert bytes(s) == _lib.PACK_SCAN(1, 2, 3, 2, *seq, 21, 22, 23, 31, 32, 33, 34, 35)
+    values = list(range(1, 25))
+    p = _lib.Policy(*values)
+    packed = _lib.PACK_POLICY(*values)
+    assert len(packed) == C.sizeof(p)
+    back = _lib.Policy.from_buffer_copy(packed)
+    for name, _ in _lib.Policy._fields_:                        # (the padding's bytes may be anything)
+        assert getattr(back, name) == getattr(p, name), name
+
+
 def _scan(**change):
     s = _lib.Scan(2, 3, 4, 0, _lib.SeqRef(64, 12, 4), _lib.SeqRef(64, 12, 4), None, None, 0, 0, None)
     for k, v in change.items():
