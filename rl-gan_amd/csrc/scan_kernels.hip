@@ -687,7 +687,9 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // A cut costs a second read of two tensors, idle CUs cost bandwidth.  Measured on an MI355X with 256, 512, 1024, 2048 workgroups
 // wanted: 65536 steps of 512 units forward fp32 161, 145, 149, 154 us, 16385 of 3000 backward bf16 257, 223, 231, 237; and with 256 or
-// more workgroups of units (1024 steps of 32768 units bf16: 46 us) a cut loses (70 us in two segments).
+// more workgroups of units (1024 steps of 32768 units bf16: 46 us) a cut loses (70 us in two segments).  Few steps are not worth a second
+// launch: whole / cut, 1024 units fp32 forward 100 steps 5.0 / 6.8 us, 200 8.0 / 6.9 (and 4 us less of the host's time), 400 12.7 / 7.1;
+// backward 8.2 / 8.8, 13.2 / 8.7, 22.8 / 9.0.
 // The chain reads everything once but has workgroups wait for each other.  What the 256 MB cache holds is cheap to read twice, the
 // rest is not: cut / chained 36 / 39 us for 100 MB (4096 steps of 4096 units bf16 forward), 61 / 77 for 246 MB (20000 of 1024
 // backward), 141 / 102 for 402 MB (65536 of 512 fp32 forward), 211 / 168 for 590 MB (16385 of 3000 bf16 backward), 213 / 150 for 737 MB
@@ -696,7 +698,8 @@ inline Plan plan(int batch, int length, int width, int size, int vec, bool backw
   constexpr int WANT = 512;
   const int64_t units = (int64_t)batch * width, bytes = (backward ? 6 : 3) * size * units * length;
   Plan p{is_serial(units, length, size), false, vec, backward ? CHAIN_BACKWARD : CHAIN_FORWARD, {(int)cdiv(units / vec, 64), 0, 0, false, nullptr}};
-  const int64_t segments = p.cut.tiles >= WANT / 2 ? 1 : cdiv(WANT, p.cut.tiles), steps = cdiv(cdiv(length, segments), TILE) * TILE;
+  const bool whole = p.cut.tiles >= WANT / 2 || length <= (backward ? 128 : 256);
+  const int64_t segments = whole ? 1 : cdiv(WANT, p.cut.tiles), steps = cdiv(cdiv(length, segments), TILE) * TILE;
   p.cut.segment = (int)steps;
   p.cut.segments = (int)cdiv(length, steps);
   p.cut.runs = p.cut.segments == 1 && width * size % 128 != 0;
