@@ -393,7 +393,7 @@ __global__ __launch_bounds__(SWEEP) void policy_swept_kernel(Policy P, const T* 
   }
 }
 
-// Several workgroups a row (where there are fewer rows than CUs: 32 x 32001 fp16 in 16 pieces 6.2 + 5.6 us, a workgroup a row took 100), each on `piece` columns: first their statistics, then (the row's joined by each for itself) the gradient
+// Several workgroups a row (few rows of many columns: latency, 32 x 100000 bf16 7 + 7 us), each on `piece` columns: first their statistics, then (the row's joined by each for itself) the gradient
 template <typename T, int N>
 __global__ __launch_bounds__(SWEEP) void policy_piece_kernel(Policy P, const T* logits, int piece, Stats* pieces, float* z_action) {
   __shared__ Stats sh[SWEEP / 64];
@@ -470,11 +470,14 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr int MAX_CUTS = 64;
 
 struct Cuts { int count, piece; };
-// enough workgroups for two a CU, each with a vector of every thread at least; measured without a difference from 256 to 2048
+// A second pass and a third launch pay for a shared row only where it is wide and rows are few: a workgroup a row / shared, bf16 with
+// gradient, 32 rows of 17000 columns 9.2 / 13.1 us, of 50000 15.2 / 14.8, of 100000 22.1 / 16.2; 128 rows of 100000 24.7 / 25.8, in fp32,
+// where such a row does not fit a CU's registers, 46.2 / 34.6; 200 rows 48.5 / 47.2.  Pieces for two workgroups a CU, each with a vector of
+// every thread at least (no difference from 256 to 2048 workgroups).
 inline Cuts cuts_of(int64_t rows, int vocab, int type) {
   constexpr int WANT = 512;
   const int n = type == TYPE_F32 ? 4 : 8, step = SWEEP * n, columns = vocab + n - 1;      // step: a vector of every thread; n - 1: the skew
-  if (rows >= WANT / 2 || vocab <= step) return {1, vocab};
+  if (vocab <= 49152 || rows > (columns > 1024 * n * 16 ? 128 : 64)) return {1, vocab};
   const int64_t count = std::min<int64_t>(std::min<int64_t>(cdiv(WANT, rows), cdiv(columns, step)), MAX_CUTS);
   const int piece = (int)(cdiv(cdiv(columns, count), step) * step);
   return {(int)cdiv(columns, piece), piece};

@@ -119,10 +119,16 @@ def test_widths(vocab, kind):
 
 
 @pytest.mark.parametrize("kind,vocab", [("fp32", 33000), ("bf16", 49999), ("bf16", 70001), ("fp16", 131072), ("fp32", 140001)])
-@pytest.mark.parametrize("rows", [3, 9])
+@pytest.mark.parametrize("rows", [3, 9, 70])
 def test_wide_rows(rows, vocab, kind):
     s = _inputs(rows, vocab, kind, 2, legal=rows == 9, pad=3)
-    _check(s, _call(s), _reference(s))
+    got = _call(s)
+    some = slice(0, 9)                                          # (what the oracle has time for)
+    part = {k: v if v is None else v[some] for k, v in s.items()}
+    ref = _reference(part)
+    if rows > 9:
+        got = R.PolicyLoss(_call(part).loss, got.logp[some], got.entropy[some], got.kl[some], got.dlogits[some])
+    _check(part, got, ref)
 
 
 @pytest.mark.parametrize("rows", [1, 2, 300, 1500])
@@ -292,7 +298,7 @@ def test_no_rows():
     assert float(got.loss) == 0 and got.dlogits.shape == (0, 8) and got.logp.shape == (0,)
 
 
-@pytest.mark.parametrize("rows,vocab", [(500, 18), (3, 40000), (700, 3001)])
+@pytest.mark.parametrize("rows,vocab", [(500, 18), (3, 40000), (3, 90000), (700, 3001)])
 def test_captured_graphs_and_streams(rows, vocab):
     """Two captured graphs and eager calls in turn: every replay gives the eager result on the inputs of its time."""
     a, b = _inputs(rows, vocab, "fp32", 13), _inputs(rows, vocab, "bf16", 14, legal=True)
