@@ -207,13 +207,14 @@ __device__ __forceinline__ void write_grad(const Policy& P, const Words<T, N>& v
 // through LDS where it has several waves); then one thread a row finishes it, those of a workgroup side by side: with a row a
 // wave and K = 1 the 64-bit arithmetic of a single lane took more time than the row's memory (1.5 million rows of 64 bf16 logits 280
 // us, side by side 143).  Bound by memory up to some 16000 columns (12207 x 16384 bf16 with gradient 153 us on an MI355X, 5.2 TB/s), beyond
-// by the few rows that fit a CU (4001 x 49999 197 us, 4.1).  parts: one sum of row losses a workgroup.
+// by the few rows that fit a CU (4001 x 49999 176 us, 4.5).  parts: one sum of row losses a workgroup.
 template <typename T, int N, int C, int GROUP, int K, bool GRAD>
 __global__ __launch_bounds__(GROUP > 256 ? GROUP : 256, N * C * K * sizeof(T) > 128 ? 4 : K > 1 || N * C * K * sizeof(T) > 64 ? 5 : 6)
 void policy_held_kernel(Policy P, const T* logits, T* dlogits, double* parts) {
   constexpr int THREADS = GROUP > 256 ? GROUP : 256, ROWS = THREADS / GROUP * K, WAVES = GROUP > 64 ? GROUP / 64 : 1;
   static_assert(WAVES == 1 || K == 1, "a row of several waves is alone in its workgroup");
   static_assert(ROWS <= THREADS, "a thread finishes one row");
+  __shared__ float sh_max[WAVES];
   __shared__ Stats sh[ROWS * WAVES];
   __shared__ RowGrad sh_row[ROWS];
   __shared__ double sh_loss[4];
@@ -234,9 +235,8 @@ void policy_held_kernel(Policy P, const T* logits, T* dlogits, double* parts) {
   }
   const int64_t my_row = row0 + threadIdx.x;                          // the row that this thread finishes
   const bool mine = threadIdx.x < ROWS && my_row < P.rows;
-  constexpr bool AHEAD = GROUP <= 256;                                // (more threads have no registers left for it)
-  RowIn in;
-  if (AHEAD && mine) {
+  RowIn in;                                                           // (read ahead: behind the sums it cost a row 10 % of its time)
+  if (mine) {
     in = row_in(P, my_row);
     in.z_action = logit_of(P, logits + my_row * P.ld, in.action);
   }
@@ -252,10 +252,10 @@ void policy_held_kernel(Policy P, const T* logits, T* dlogits, double* parts) {
     } else {
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) st.m = fmaxf(st.m, __shfl_xor(st.m, o));
-      if ((threadIdx.x & 63) == 0) sh[me / 64].m = st.m;
+      if ((threadIdx.x & 63) == 0) sh_max[me / 64] = st.m;
       __syncthreads();
 #pragma unroll 4
-      for (int w = 0; w < WAVES; ++w) st.m = fmaxf(st.m, sh[w].m);
+      for (int w = 0; w < WAVES; ++w) st.m = fmaxf(st.m, sh_max[w]);
       st.m = uniform(st.m);
     }
     if (is_far(st.m, P.scale)) {
@@ -269,30 +269,26 @@ void policy_held_kernel(Policy P, const T* logits, T* dlogits, double* parts) {
       if (c * GROUP * N + wave0 < P.vocab + skew[k]) { add_to(st, v[k][c], shift, P.scale); v[k][c].pin(); }
 #pragma unroll
     for (int o = (GROUP < 64 ? GROUP : 64) / 2; o > 0; o >>= 1) { st.s += __shfl_xor(st.s, o); st.t += __shfl_xor(st.t, o); }
-    if constexpr (WAVES > 1) __syncthreads();                         // the maxima have been read
     if ((WAVES > 1 ? threadIdx.x & 63 : me) == 0) sh[WAVES > 1 ? me / 64 : slot + k] = st;
   }
   __syncthreads();
   double loss = 0;
   if (mine) {
-    if (!AHEAD) {
-      in = row_in(P, my_row);
-      in.z_action = logit_of(P, logits + my_row * P.ld, in.action);
-    }
     Stats st = sh[threadIdx.x * WAVES];
 #pragma unroll 4
     for (int w = 1; w < WAVES; ++w) { st.s += sh[w].s; st.t += sh[w].t; }
     sh_row[threadIdx.x] = finish_row(P, my_row, in, st, true, loss);
   }
-  if (threadIdx.x < 256) {
-    if constexpr (ROWS > 1) {
+  if constexpr (ROWS == 1) {
+    if (mine) parts[blockIdx.x] = loss;
+    __syncthreads();
+  } else {
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) loss += __shfl_xor(loss, o);
-    }
+    for (int o = 32; o > 0; o >>= 1) loss += __shfl_xor(loss, o);
     if ((threadIdx.x & 63) == 0) sh_loss[threadIdx.x >> 6] = loss;
+    __syncthreads();
+    if (threadIdx.x == 0) parts[blockIdx.x] = ((sh_loss[0] + sh_loss[1]) + sh_loss[2]) + sh_loss[3];
   }
-  __syncthreads();
-  if (threadIdx.x == 0) parts[blockIdx.x] = ((sh_loss[0] + sh_loss[1]) + sh_loss[2]) + sh_loss[3];
   if constexpr (GRAD) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -532,9 +528,9 @@ void launch_rows(const Policy& P, const rlgan_policy_t* p, void* workspace, int6
   if (narrow <= 1024) HELD(4, 4, 64, V / 2);
   if (narrow <= 2048) HELD(4, 8, 64, 1);
   if (p->dlogits) {
-    // Several rows a CU hide each other's reductions, so a row takes as few threads as its registers allow.  Measured on an
-    // MI355X, bf16, gradient read and write of 200 million logits: 16384 columns in 256 threads 161 us, in 1024 226;
-    // 32768 in 512 161, 256 169, 1024 187; 49999 in 512 200, 256 241, 1024 202.
+    // Several rows a CU hide each other's reductions; a row takes no more threads than its registers ask for, but enough to be
+    // through quickly.  Measured on an MI355X, bf16, gradient read and write of 200 million logits: 16384 columns in 256 threads 161
+    // us, in 1024 226; 32768 in 512 154, 256 183, 1024 187; 49999 in 512 176, 256 201, 1024 202; 65536 in 512 162.
     if (columns <= 256 * W * 4) HELD(W, 4, 256, 1);
     if (columns <= 256 * W * 8) HELD(W, 8, 256, 1);
     if (columns <= 512 * W * 8) HELD(W, 8, 512, 1);
