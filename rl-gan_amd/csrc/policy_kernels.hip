@@ -305,7 +305,7 @@ void policy_held_kernel(Policy P, const T* logits, T* dlogits, double* parts) {
 }
 
 // ---- rows that are swept ------------------------------------------------------------------------------------------------
-// Wider rows, rows without a gradient to write, and rows that several workgroups share: a sweep over some of a row's columns keeps
+// Wider rows, and rows that several workgroups share: a sweep over some of a row's columns keeps
 // a running maximum and moves the sums when it grows; the gradient's sweep reads them again, from the caches.  Bound by memory: 1027 x
 // 131072 fp32 without gradient 100 us (5.4 TB/s on an MI355X), 762 x 131072 fp32 with one 241 us (3.3 of the 5.0 that reading once would
 // allow: the row does not fit a CU's registers).
@@ -527,7 +527,9 @@ void launch_rows(const Policy& P, const rlgan_policy_t* p, void* workspace, int6
   if (narrow <= 512) HELD(4, 2, 64, V);
   if (narrow <= 1024) HELD(4, 4, 64, V / 2);
   if (narrow <= 2048) HELD(4, 8, 64, 1);
-  if (p->dlogits) {
+  // (Without a gradient too: held / swept, bf16, 200 million logits read, rows of 3000 columns 166 / 502 us, 16384 74 / 118, 49999 90 / 90;
+  // fp32 rows of 49999, which take 1024 threads, 95 / 80.)
+  if (p->dlogits || columns <= 512 * W * 16) {
     // Several rows a CU hide each other's reductions; a row takes no more threads than its registers ask for, but enough to be
     // through quickly.  Measured on an MI355X, bf16, gradient read and write of 200 million logits: 16384 columns in 256 threads 161
     // us, in 1024 226; 32768 in 512 154, 256 183, 1024 187; 49999 in 512 176, 256 201, 1024 202; 65536 in 512 162.

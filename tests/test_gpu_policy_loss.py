@@ -126,6 +126,7 @@ def test_wide_rows(rows, vocab, kind):
     some = slice(0, 9)                                          # (what the oracle has time for)
     part = {k: v if v is None else v[some] for k, v in s.items()}
     ref = _reference(part)
+    _check(part, _call(part, grad=False), ref, grad=False)
     if rows > 9:
         got = R.PolicyLoss(_call(part).loss, got.logp[some], got.entropy[some], got.kl[some], got.dlogits[some])
     _check(part, got, ref)
