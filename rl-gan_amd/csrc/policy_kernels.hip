@@ -66,6 +66,7 @@ __device__ __forceinline__ float settled(float z, float m) {
 // does this once.  `writer`: the thread that leaves the row's results; loss: the row's weighted share.
 // Rows left out (action < 0, weight 0, an action that is not allowed): zeros everywhere.  An action >= vocab: NaN everywhere.
 __device__ RowGrad finish_row(const Policy& P, int64_t row, const RowIn& in, const Stats& st, bool writer, double& loss) {
+#pragma clang fp contract(off)                       // (a row's bits do not depend on how many rows a thread holds)
   const double w = P.weights ? (double)in.weight : P.row_weight;
   RowGrad g{0.f, 0.f, 0.f, 0.f, -1};
   double logp = 0, entropy = 0, kl = 0;
@@ -171,20 +172,21 @@ template <typename T, int N> __device__ __forceinline__ void add_to(Stats& a, co
   for (int i = 0; i < N; ++i) {
     const float x = __builtin_fmaf(v.get(i), scale, -shift), e = __builtin_amdgcn_exp2f(x);
     a.s += e;
-    a.t += fmaxf(x, -1e4f) * e;
+    a.t = __builtin_fmaf(fmaxf(x, -1e4f), e, a.t);
   }
 }
 
 // gradients for columns j .. j + N - 1, written to d (the row's)
 template <typename T, int N>
 __device__ __forceinline__ void write_grad(const Policy& P, const Words<T, N>& v, int j, const RowGrad& g, T* d) {
+#pragma clang fp contract(off)
   if (j >= P.vocab) return;
   Words<T, N> out;
   float val[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float y = __builtin_fmaf(v.get(i), P.scale, -g.shift);
-    val[i] = __builtin_amdgcn_exp2f(y) * (g.a0 + g.a1 * fmaxf(y, -1e4f));
+    val[i] = __builtin_amdgcn_exp2f(y) * __builtin_fmaf(g.a1, fmaxf(y, -1e4f), g.a0);
   }
   const int at = inside<N>(P, j);
   if (g.action < 0) {                                    // a row left out: zeros; no such action: NaN
@@ -206,10 +208,11 @@ __device__ __forceinline__ void write_grad(const Policy& P, const Words<T, N>& v
 // GROUP threads hold K rows, each in C vectors of N a thread: read once, written once.  A row's sums are joined by shuffles (and
 // through LDS where it has several waves); then one thread a row finishes it, those of a workgroup side by side: with a row a
 // wave and K = 1 the 64-bit arithmetic of a single lane took more time than the row's memory (1.5 million rows of 64 bf16 logits 280
-// us, side by side 143).  Bound by memory up to some 16000 columns (12207 x 16384 bf16 with gradient 153 us on an MI355X, 5.2 TB/s), beyond
+// us, side by side 114).  Bound by memory up to some 16000 columns (12207 x 16384 bf16 with gradient 153 us on an MI355X, 5.2 TB/s), beyond
 // by the few rows that fit a CU (4001 x 49999 176 us, 4.5).  parts: one sum of row losses a workgroup.
+// (The second bound: waves a SIMD that the row's registers leave room for.)
 template <typename T, int N, int C, int GROUP, int K, bool GRAD>
-__global__ __launch_bounds__(GROUP > 256 ? GROUP : 256, N * C * K * sizeof(T) > 128 ? 4 : K > 1 || N * C * K * sizeof(T) > 64 ? 5 : 6)
+__global__ __launch_bounds__(GROUP > 256 ? GROUP : 256, N * C * K * sizeof(T) > 128 ? 4 : N * C * K * sizeof(T) > 64 || K > 1 ? 5 : 6)
 void policy_held_kernel(Policy P, const T* logits, T* dlogits, double* parts) {
   constexpr int THREADS = GROUP > 256 ? GROUP : 256, ROWS = THREADS / GROUP * K, WAVES = GROUP > 64 ? GROUP / 64 : 1;
   static_assert(WAVES == 1 || K == 1, "a row of several waves is alone in its workgroup");
@@ -514,19 +517,31 @@ void launch_rows(const Policy& P, const rlgan_policy_t* p, void* workspace, int6
     return;
   }
 #define HELD(N, C, GROUP, K) return launch_held<T, N, C, GROUP, K>(P, p, parts, n_parts, st)
-  constexpr int V = sizeof(T) == 4 ? 2 : 4;
   // room for the skew of rows that begin anywhere
   const bool aligned = (uintptr_t)p->logits % 16 == 0 && (rows == 1 || p->ld % W == 0);
   const int64_t columns = vocab + (aligned ? 0 : W - 1), narrow = W == 4 ? columns : vocab;
+  // A row takes few threads with several vectors each: 100 million bf16 logits with gradient, rows of 256 columns in 16 threads 90 us, in
+  // 32 114, in 64 (vectors of 4) 149; 1024 in 32 82, in 64 88 (vectors of 4: 107); 3000 in 64 91, in 256 115; 50 million fp32 of 180
+  // columns in 16 87, in 64 149.
   if (vocab < 4) HELD(1, 1, 4, 4);
   if (narrow <= 16) HELD(4, 1, 4, 4);
   if (narrow <= 32) HELD(4, 1, 8, 4);
-  if (narrow <= 64) HELD(4, 1, 16, 2 * V);
-  if (narrow <= 128) HELD(4, 1, 32, 2 * V);
-  if (narrow <= 256) HELD(4, 1, 64, 2 * V);
-  if (narrow <= 512) HELD(4, 2, 64, V);
-  if (narrow <= 1024) HELD(4, 4, 64, V / 2);
-  if (narrow <= 2048) HELD(4, 8, 64, 1);
+  if constexpr (W == 8) {
+    if (columns <= 64) HELD(8, 1, 8, 4);
+    if (columns <= 128) HELD(8, 2, 8, 4);
+    if (columns <= 256) HELD(8, 2, 16, 2);
+    if (columns <= 512) HELD(8, 4, 16, 2);
+    if (columns <= 1024) HELD(8, 4, 32, 1);
+    if (columns <= 2048) HELD(8, 8, 32, 1);
+    if (columns <= 4096) HELD(8, 8, 64, 1);
+  } else {
+    if (columns <= 64) HELD(4, 2, 8, 4);
+    if (columns <= 128) HELD(4, 2, 16, 2);
+    if (columns <= 256) HELD(4, 4, 16, 1);
+    if (columns <= 512) HELD(4, 4, 32, 1);
+    if (columns <= 1024) HELD(4, 4, 64, 1);
+    if (columns <= 2048) HELD(4, 8, 64, 1);
+  }
   // (Without a gradient too: held / swept, bf16, 200 million logits read, rows of 3000 columns 166 / 502 us, 16384 74 / 118, 49999 90 / 90;
   // fp32 rows of 49999, which take 1024 threads, 95 / 80.)
   if (p->dlogits || columns <= 512 * W * 16) {

@@ -106,7 +106,8 @@ def _check(s, got, ref, grad=True, **more):
     assert np.all(g[~used] == 0)
 
 
-VOCABS = [1, 2, 3, 4, 7, 17, 18, 31, 64, 65, 200, 256, 500, 1000, 2049, 4097, 8191, 16385]
+VOCABS = [1, 2, 3, 4, 7, 13, 16, 17, 18, 29, 31, 32, 57, 63, 64, 65, 121, 128, 129, 200, 255, 256, 257, 500, 512, 513, 1000, 1024, 1025, 2041, 2048, 2049,
+          4089, 4096, 4097, 8191, 8192, 8193, 16385, 24577]
 
 
 @pytest.mark.parametrize("kind", sorted(TYPES))
@@ -130,6 +131,33 @@ def test_wide_rows(rows, vocab, kind):
     if rows > 9:
         got = R.PolicyLoss(_call(part).loss, got.logp[some], got.entropy[some], got.kl[some], got.dlogits[some])
     _check(part, got, ref)
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("vocab,rows", [(2, 140001), (9, 140001), (27, 70003), (50, 70003), (64, 70003), (111, 70003), (200, 33001), (256, 33001), (450, 20001),
+                                        (900, 9001), (1500, 5001)])
+def test_many_rows(rows, vocab, kind):
+    """Groups of threads that hold several rows: every row has the bits that it has in a call of few rows; the loss is their sum (in
+    64 bits but for the last rounding)."""
+    g = torch.Generator(device="cuda").manual_seed(20)
+    z = torch.randn(rows, vocab + 1, generator=g, device="cuda").to(TYPES[kind])[:, :vocab]
+    a = torch.randint(-1, vocab, (rows,), generator=g, device="cuda")
+    s = dict(logits=z, actions=a, old_logp=torch.full((rows,), -float(np.log(vocab)), device="cuda"),
+             advantages=torch.randn(rows, generator=g, device="cuda") + 1, weights=torch.rand(rows, generator=g, device="cuda"), ref_logp=None,
+             legal=torch.rand(rows, vocab, generator=g, device="cuda") > 0.2 if vocab == 50 else None)
+    got = _call(s)
+    total = 0.0
+    for at in list(range(0, rows, max(1, rows // 7)))[:8]:
+        some = slice(at, at + 40)
+        part = {k: v if v is None else v[some] for k, v in s.items()}
+        few = _call(part)
+        for p, q in zip(got[1:], few[1:]):
+            assert torch.equal(p[some], q)
+    first = {k: v if v is None else v[:20] for k, v in s.items()}
+    _check(first, _call(first), _reference(first))
+    for at in range(0, rows, 1000):
+        total += float(_call({k: v if v is None else v[at:at + 1000] for k, v in s.items()}, grad=False).loss)
+    assert abs(total - float(got.loss)) <= 2 * U * abs(total) + (rows / 1000 + 1) * U * abs(total)
 
 
 @pytest.mark.parametrize("rows", [1, 2, 300, 1500])
