@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256) void scan_serial_bwd(Units u, Seq<const T> dh,
 // flight meanwhile, and 8 waves work on units that are one dependent chain.  Where there are too few units to fill the chip the
 // time axis is cut into segments: a first kernel folds every segment to its map, and the walk of a segment begins with the
 // composition of the maps before it.  Bound by memory: 1024 steps of 32768 units bf16 forward 46 us (4.4 TB/s on an MI355X, where a copy
-// runs at 5.0), 200 steps of 25800 fp32 units backward 36 us (3.4; seven tiles a workgroup leave a ramp and a tail).
+// runs at 5.0), 200 steps of 25800 fp32 units backward 33 us (3.8; seven tiles a workgroup leave a ramp and a tail).
 
 constexpr int WAVES = 8, STEPS = 8, TILE = WAVES * STEPS;
 // the backward walk has twice the tensors to hold: 4 steps a wave leave room for two workgroups a CU (16385 steps of 3000 units bf16
@@ -141,13 +141,14 @@ __device__ __forceinline__ Place place(int tiles, bool runs) {
 template <int VEC> struct Lanes {                // the units of a lane
   int64_t unit;                                  // first of them, counted through the batch
   int b, d, len;
-  bool real;
+  bool real, one_row;                            // one_row: all lanes of the wave have the same b
   __device__ __forceinline__ Lanes(const Units& u, int tile, bool mask) {
     const int wv = u.width / VEC, total = u.batch * wv;
     const int i = tile * 64 + (threadIdx.x & 63), k = min(i, total - 1);   // lanes behind the last repeat it and write nothing
     real = i < total;
     b = k / wv; d = (k - b * wv) * VEC;
     unit = (int64_t)b * u.width + d;
+    one_row = __all(b == __builtin_amdgcn_readfirstlane(b));
     len = mask && u.lengths ? min(max(u.lengths[b], 0), u.length) : u.length;
   }
 };
@@ -158,13 +159,29 @@ __device__ __forceinline__ void load_steps(Words<T, VEC> (&v)[COUNT], const T* p
 #pragma unroll
   for (int i = 0; i < COUNT; ++i) v[i].load(p + min(max(t0 + i, 0), length - 1) * stride);
 }
-template <int COUNT = STEPS> __device__ __forceinline__ uint32_t load_starts(const uint8_t* p, int64_t stride, int t0, int length) {
-  uint32_t bits = 0;
-  if (p) {
+// The start flags of COUNT steps, as loaded: `bits` is asked for where they are used, so that nothing waits for them before (flags
+// joined to bits at once cost the walk of 32768 bf16 units 4 us of 47).
+template <int COUNT> struct Starts {
+  uint8_t v[COUNT];
+  __device__ __forceinline__ void load(const uint8_t* p, int64_t stride, int t0, int length) {
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) bits |= (p[min(t0 + i, length - 1) * stride] ? 1u : 0u) << i;
+    for (int i = 0; i < COUNT; ++i) v[i] = p ? p[min(t0 + i, length - 1) * stride] : 0;
   }
-  return bits;
+  __device__ __forceinline__ uint32_t bits() const {
+    uint32_t b = 0;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) b |= (v[i] ? 1u : 0u) << i;
+    return b;
+  }
+};
+// the same where there is nothing to wait with: a wave whose units belong to one batch row reads a step a lane
+template <int COUNT> __device__ __forceinline__ uint32_t starts_now(const uint8_t* p, bool one_row, int64_t stride, int t0, int length) {
+  const int lane = threadIdx.x & 63;
+  if (!p) return 0;
+  if (one_row) return (uint32_t)__ballot(lane < COUNT && p[min(t0 + min(lane, COUNT - 1), length - 1) * stride] != 0);
+  Starts<COUNT> s;
+  s.load(p, stride, t0, length);
+  return s.bits();
 }
 
 // the map of one step, forward: folds it behind m
@@ -196,21 +213,22 @@ __global__ __launch_bounds__(WAVES * 64) void scan_fold_kernel(Units u, Seq<cons
 #pragma unroll
   for (int k = 0; k < VEC; ++k) m[k] = {1.f, 0.f};
   Words<T, VEC> zv[2][STEPS], xv[2][STEPS];
-  uint32_t st[2] = {0, 0};
+  Starts<STEPS> st[2];
   const int n = end > begin ? (end - begin + STEPS - 1) / STEPS : 0;
   const int first = BACK ? begin + (n - 1) * STEPS : begin, hop = BACK ? -STEPS : STEPS;
-  if (n > 0) { load_steps(zv[0], zp, z.t, first, u.length); load_steps(xv[0], xp, x_or_dh.t, first, u.length); st[0] = load_starts(sp, u.starts_t, first, u.length); }
+  if (n > 0) { load_steps(zv[0], zp, z.t, first, u.length); load_steps(xv[0], xp, x_or_dh.t, first, u.length); st[0].load(sp, u.starts_t, first, u.length); }
   for (int j = 0; j < n; j += 2) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (j + half >= n) break;
       const int t0 = first + (j + half) * hop, nt = j + half + 1 < n ? t0 + hop : t0;
       load_steps(zv[half ^ 1], zp, z.t, nt, u.length); load_steps(xv[half ^ 1], xp, x_or_dh.t, nt, u.length);
-      st[half ^ 1] = load_starts(sp, u.starts_t, nt, u.length);
+      st[half ^ 1].load(sp, u.starts_t, nt, u.length);
+      const uint32_t bits = MASK ? st[half].bits() : 0;
 #pragma unroll
       for (int q = 0; q < STEPS; ++q) {
         const int i = BACK ? STEPS - 1 - q : q, t = t0 + i;
-        const bool start = MASK && ((st[half] >> i) & 1), live = t < (MASK ? min(me.len, end) : end);
+        const bool start = MASK && ((bits >> i) & 1), live = t < (MASK ? min(me.len, end) : end);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
           float f, take;
@@ -280,7 +298,8 @@ __global__ __launch_bounds__(WAVES * 64) void scan_walk_fwd(Units u, Seq<const T
   Words<T, VEC> zn[STEPS], xn[STEPS];
   load_steps(zn, zp, z.t, begin + wave * STEPS, u.length);
   load_steps(xn, xp, x.t, begin + wave * STEPS, u.length);
-  uint32_t stn = load_starts(sp, u.starts_t, begin + wave * STEPS, u.length);
+  Starts<STEPS> stn;
+  stn.load(sp, u.starts_t, begin + wave * STEPS, u.length);
   if (cut.segments > 1) enter_segment<VEC, false>(me, cut, seg, units, sh[0], s);
   else {
 #pragma unroll
@@ -290,7 +309,7 @@ __global__ __launch_bounds__(WAVES * 64) void scan_walk_fwd(Units u, Seq<const T
   for (int tile = begin; tile < end; tile += TILE, turn ^= 1) {
     const int t0 = tile + wave * STEPS;
     float take[STEPS][VEC], xf[STEPS][VEC];
-    const uint32_t st = stn;
+    const uint32_t st = MASK ? stn.bits() : 0;
     Map m[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) m[k] = {1.f, 0.f};
@@ -306,7 +325,7 @@ __global__ __launch_bounds__(WAVES * 64) void scan_walk_fwd(Units u, Seq<const T
     if (tile + TILE < end) {
       load_steps(zn, zp, z.t, t0 + TILE, u.length);
       load_steps(xn, xp, x.t, t0 + TILE, u.length);
-      stn = load_starts(sp, u.starts_t, t0 + TILE, u.length);
+      stn.load(sp, u.starts_t, t0 + TILE, u.length);
     }
 #pragma unroll
     for (int k = 0; k < VEC; ++k) sh[turn][wave][lane * VEC + k] = m[k];
@@ -358,13 +377,13 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_walk_bwd(Units u, Seq<cons
   const int begin = seg * cut.segment, end = min(begin + cut.segment, u.length);
   const int last = begin + (end - begin - 1) / BACK_TILE * BACK_TILE;
   Words<T, VEC> zn[BACK_STEPS], xn[BACK_STEPS], gn[BACK_STEPS], hn[BACK_STEPS];
-  uint32_t stn;
+  Starts<BACK_STEPS> stn;
   auto fetch = [&](int t0) {
     load_steps(zn, zp, z.t, t0, u.length);
     load_steps(gn, gp, dh.t, t0, u.length);
     load_steps(xn, xp, x.t, t0, u.length);
     load_steps(hn, hp, h.t, t0 - 1, u.length);
-    stn = load_starts<BACK_STEPS>(sp, u.starts_t, t0, u.length);
+    stn.load(sp, u.starts_t, t0, u.length);
   };
   fetch(last + wave * BACK_STEPS);
   if (cut.segments > 1) enter_segment<VEC, true>(me, cut, seg, units, sh[0], c);
@@ -376,7 +395,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_walk_bwd(Units u, Seq<cons
   for (int tile = last; tile >= begin; tile -= BACK_TILE, turn ^= 1) {
     const int t0 = tile + wave * BACK_STEPS;
     Words<T, VEC> xv[BACK_STEPS], gv[BACK_STEPS], hv[BACK_STEPS];
-    const uint32_t st = stn;
+    const uint32_t st = MASK ? stn.bits() : 0;
     float fs[BACK_STEPS][VEC], takes[BACK_STEPS][VEC];
     Map m[VEC];
 #pragma unroll
@@ -435,7 +454,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_walk_bwd(Units u, Seq<cons
 // is not there yet is all ones: no other memory needs ordering.  Every wait ends: chunks are numbered by a ticket that a workgroup
 // draws when it runs; it waits for the maps of chunks with smaller tickets, whose workgroups run and hand those on without waiting
 // for anything, and at most for the state of one such chunk, which by the same argument from the first chunk on is handed on too.  Bound by what the look-back
-// leaves unhidden with two workgroups a CU: 65536 steps of 512 units fp32 forward 102 us (3.9 TB/s), 16385 of 3000 bf16 backward 168
+// leaves unhidden with two workgroups a CU: 65536 steps of 512 units fp32 forward 99 us (4.1 TB/s), 16385 of 3000 bf16 backward 168
 // (3.5).
 
 // Steps of a wave in a chunk, forward and backward.  More of them wait less for each other, fewer leave room for a second workgroup
@@ -568,7 +587,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_chain_fwd(Units u, Seq<con
   Words<T, VEC> zv[ST], xv[ST];
   load_steps(zv, zp, z.t, t0, u.length);
   load_steps(xv, xp, x.t, t0, u.length);
-  const uint32_t st = load_starts<ST>(MASK && u.starts ? u.starts + me.b * u.starts_b : nullptr, u.starts_t, t0, u.length);
+  const uint32_t st = starts_now<ST>(MASK && u.starts ? u.starts + me.b * u.starts_b : nullptr, me.one_row, u.starts_t, t0, u.length);
   Map m[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) m[k] = {1.f, 0.f};
@@ -625,7 +644,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_chain_bwd(Units u, Seq<con
   load_steps(gv, dh.p + me.b * dh.b + me.d, dh.t, t0, u.length);
   load_steps(xv, x.p + me.b * x.b + me.d, x.t, t0, u.length);
   load_steps(hv, h.p + me.b * h.b + me.d, h.t, t0 - 1, u.length);
-  const uint32_t st = load_starts<ST>(MASK && u.starts ? u.starts + me.b * u.starts_b : nullptr, u.starts_t, t0, u.length);
+  const uint32_t st = starts_now<ST>(MASK && u.starts ? u.starts + me.b * u.starts_b : nullptr, me.one_row, u.starts_t, t0, u.length);
   Map m[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) m[k] = {1.f, 0.f};
