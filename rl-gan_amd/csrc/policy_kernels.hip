@@ -209,7 +209,7 @@ __device__ __forceinline__ void write_grad(const Policy& P, const Words<T, N>& v
 // through LDS where it has several waves); then one thread a row finishes it, those of a workgroup side by side: with a row a
 // wave and K = 1 the 64-bit arithmetic of a single lane took more time than the row's memory (1.5 million rows of 64 bf16 logits 280
 // us, side by side 114).  Bound by memory up to some 16000 columns (12207 x 16384 bf16 with gradient 153 us on an MI355X, 5.2 TB/s), beyond
-// by the few rows that fit a CU (4001 x 49999 176 us, 4.5).  parts: one sum of row losses a workgroup.
+// by the few rows that fit a CU (4001 x 49999 171 us, 4.7).  parts: one sum of row losses a workgroup.
 // (The second bound: waves a SIMD that the row's registers leave room for.)
 template <typename T, int N, int C, int GROUP, int K, bool GRAD>
 __global__ __launch_bounds__(GROUP > 256 ? GROUP : 256, N * C * K * sizeof(T) > 128 ? 4 : N * C * K * sizeof(T) > 64 || K > 1 ? 5 : 6)
