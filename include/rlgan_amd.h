@@ -38,8 +38,8 @@ enum { RLGAN_NET_ACTOR = 0, RLGAN_NET_CRITIC = 1, RLGAN_NET_GENERATOR = 2, RLGAN
 
 enum {
   RLGAN_E_ARG = -1,      /* null pointer / negative size */
-  RLGAN_E_DIMS = -2,     /* state/action dims outside what the kernels are built for */
-  RLGAN_E_KIND = -3,     /* unknown network kind */
+  RLGAN_E_DIMS = -2,     /* state/action dims or other sizes outside what the kernels are built for */
+  RLGAN_E_KIND = -3,     /* unknown network kind, element type or width of a state */
   RLGAN_E_NOTFULL = -4,  /* replay sample before the ring is full (Curious_GAN.py:167 assert) */
   RLGAN_E_ALIGN = -5,    /* row count / leading dimension not as documented */
   RLGAN_E_SCRATCH = -6   /* size beyond the fixed device scratch of an allocation-free entry point */
@@ -728,7 +728,8 @@ typedef struct {
   int32_t random, reserved;                /* 8 bits: codes rounded at random (1), by Philox under `seed`, or to nearest (0) */
   uint64_t seed;
 } rlgan_adamw_t;
-/* grads, grad_types: HOST arrays of n_tensors device pointers and element types (any of the three, whatever the parameter's).
+/* grads, grad_types: HOST arrays of n_tensors device pointers and element types (any of the three, whatever the parameter's),
+ * which share no memory with the parameters.
  * grad_scale: device scalar or NULL.  skip: device byte or NULL; where it is not 0 the call changes nothing. */
 int rlgan_adamw_step(const rlgan_adamw_t* a, const void* const* grads, const uint8_t* grad_types, const float* grad_scale, const uint8_t* skip,
                      void* stream);

@@ -67,21 +67,35 @@ class AdamW:
         if state_bits == 8:
             self.first_exp = torch.zeros(n // ADAMW_BLOCK, dtype=torch.uint8, device=dev)
             self.second_exp = torch.zeros_like(self.first_exp)
-        self.lr = torch.full((1,), float(lr), dtype=torch.float32, device=dev)
-        self.steps = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._lr = torch.full((1,), float(lr), dtype=torch.float32, device=dev)
+        self._steps = torch.zeros(1, dtype=torch.int32, device=dev)
         self._scalars = torch.zeros(8, dtype=torch.float32, device=dev)
         ptr = lambda t: None if t is None else t.data_ptr()
         self._state = AdamWState(len(counts), state_bits, ptr(self._records), ptr(self._chunks), self._chunk_begin.ctypes.data, ptr(self.first),
-                                 ptr(self.second), ptr(self.first_exp), ptr(self.second_exp), ptr(self.lr), ptr(self.steps), ptr(self._scalars),
+                                 ptr(self.second), ptr(self.first_exp), ptr(self.second_exp), ptr(self._lr), ptr(self._steps), ptr(self._scalars),
                                  self.betas[0], self.betas[1], self.eps, self.weight_decay, rounding == "random", 0, int(seed))
+
+    @property
+    def lr(self) -> torch.Tensor:
+        """The rate, a float32 device scalar [1]; assigning a number is `set_lr`."""
+        return self._lr
+
+    @lr.setter
+    def lr(self, value: float) -> None:
+        self.set_lr(value)
+
+    @property
+    def steps(self) -> torch.Tensor:
+        """Steps done, an int32 device counter [1]."""
+        return self._steps
 
     def set_lr(self, lr: float) -> None:
         """The rate of the following steps, those of captured graphs among them."""
-        need(lr >= 0, "lr: not negative")
-        self.lr.fill_(float(lr))
+        need(float(lr) >= 0, "lr: not negative")
+        self._lr.fill_(float(lr))
 
     def step(self, grads: Sequence[torch.Tensor], grad_scale: Optional[torch.Tensor] = None, skip: Optional[torch.Tensor] = None) -> None:
-        """One step.  grads: a gradient for every parameter, of its shape, in any of the three types.  grad_scale: float32
+        """One step.  grads: a gradient for every parameter, of its shape, in any of the three types, in memory of its own.  grad_scale: float32
         device scalar that multiplies the gradients (1 / loss scale, what clipping by a norm left).  skip: bool device scalar;
         where it is True nothing changes (gradients of a scaled loss that overflowed)."""
         need(len(grads) == len(self.params), f"{len(grads)} gradients for {len(self.params)} parameters")

@@ -38,8 +38,8 @@ const char* rlgan_error_string(int code) {
   switch (code) {
     case 0: return "ok";
     case RLGAN_E_ARG: return "null pointer or negative size";
-    case RLGAN_E_DIMS: return "state/action dimensions outside what the kernels are built for (2*s_dim+a_dim <= 16)";
-    case RLGAN_E_KIND: return "unknown network kind";
+    case RLGAN_E_DIMS: return "sizes outside what the kernels are built for (networks: state/action dimensions with 2*s_dim+a_dim <= 16)";
+    case RLGAN_E_KIND: return "unknown network kind, element type or width of a state";
     case RLGAN_E_NOTFULL: return "Memory has not been fulfilled";
     case RLGAN_E_ALIGN: return "row count or leading dimension not as documented";
     case RLGAN_E_SCRATCH: return "size beyond the fixed device scratch of the allocation-free entry point (rlgan_column_sums_noalloc: n_cols <= 256)";

@@ -715,14 +715,14 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // (4000 of 15360 fp32 forward).
 inline Plan plan(int batch, int length, int width, int size, int vec, bool backward) {
   constexpr int WANT = 512;
-  const int64_t units = (int64_t)batch * width, bytes = (backward ? 6 : 3) * size * units * length;
+  const int64_t units = (int64_t)batch * width;
   Plan p{is_serial(units, length, size), false, vec, backward ? CHAIN_BACKWARD : CHAIN_FORWARD, {(int)cdiv(units / vec, 64), 0, 0, false, nullptr}};
   const bool whole = p.cut.tiles >= WANT / 2 || length <= (backward ? 128 : 256);
   const int64_t segments = whole ? 1 : cdiv(WANT, p.cut.tiles), steps = cdiv(cdiv(length, segments), TILE) * TILE;
   p.cut.segment = (int)steps;
   p.cut.segments = (int)cdiv(length, steps);
   p.cut.runs = p.cut.segments == 1 && width * size % 128 != 0;
-  p.chained = !p.serial && p.cut.segments > 1 && bytes > CACHE;
+  p.chained = !p.serial && p.cut.segments > 1 && units * length > CACHE / ((backward ? 6 : 3) * size);
   return p;
 }
 inline Chain chain_of(const Plan& p, int length, int64_t units, void* workspace) {

@@ -137,7 +137,10 @@ def test_scale_skip_and_rate(bits):
     opt.step([torch.full_like(g, float("inf")) for g in grads], skip=torch.ones(1, dtype=torch.bool, device="cuda"))
     for a, b in zip(held, params + list(opt.state_dict().values())):
         assert torch.equal(a, b)
-    opt.set_lr(LR / 2)
+    opt.lr = LR / 2                                             # a number goes into the device scalar that the kernels read
+    assert torch.is_tensor(opt.lr) and float(opt.lr) == np.float32(LR / 2)
+    with pytest.raises(AttributeError):
+        opt.steps = 3
     opt.step(grads, skip=torch.zeros((), dtype=torch.uint8, device="cuda"))
     host.step(grads, lr=LR / 2)
     host.check(2)
