@@ -150,10 +150,13 @@ class AdamW:
             on_device(t, self.device, name)
             need(t.dtype == torch.float32 and t.shape == (self.size,), f"{name}: float32 of shape [{self.size}]")
         need(0 <= int(steps) < 1 << 31, "steps: not negative")
-        clean = [torch.zeros(max(self.size, ADAMW_BLOCK), dtype=torch.float32, device=self.device) for _ in range(2)]
+        ends = np.array([p.numel() for p in self.params], np.int64) + self.offsets[:-1]
+        gaps = np.concatenate([np.arange(a, b) for a, b in zip(ends, self.offsets[1:])] + [np.arange(self.size, self.first.numel())])
+        gaps = torch.from_numpy(gaps.astype(np.int64)).to(self.device)
+        clean = [torch.empty(self.first.numel(), dtype=torch.float32, device=self.device) for _ in range(2)]
         for to, t in zip(clean, (first, second)):
-            for a, b in zip(self.views(to), self.views(t)):
-                a.copy_(b)
+            to[:self.size].copy_(t)
+            to[gaps] = 0.0                                       # between the parameters the state stays 0
         if self.state_bits == 32:
             self.first.copy_(clean[0])
             self.second.copy_(clean[1])
