@@ -336,6 +336,24 @@ def test_captured_steps(bits):
                 assert torch.equal(a, b), turn
 
 
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_tensor_of_more_than_32_bits(bits):
+    """The last elements of a tensor of more than 2^31 step as those of a small one do, to the bit."""
+    n, tail = (1 << 31) + 64 * 1000 + 37, 64 * 200 + 37
+    p = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    rnd = torch.Generator(device="cuda").manual_seed(11)
+    p[-tail:] = torch.randn(tail, generator=rnd, device="cuda").bfloat16()
+    g[-tail:] = torch.randn(tail, generator=rnd, device="cuda").bfloat16()
+    small, small_g = p[-tail:].clone(), g[-tail:].clone()
+    big, few = R.AdamW([p], state_bits=bits, **HYPER), R.AdamW([small], state_bits=bits, **HYPER)
+    for _ in range(2):
+        big.step([g])
+        few.step([small_g])
+    assert torch.equal(p[-tail:], small) and (p[:1000] == 0).all()
+    assert torch.equal(big.first[n - tail:n], few.first[:tail]) and torch.equal(big.second[n - tail:n], few.second[:tail])
+
+
 def test_refusals():
     p = torch.zeros(10, device="cuda")
     bad = [lambda: R.AdamW([]), lambda: R.AdamW([p], state_bits=16), lambda: R.AdamW([p.cpu()]), lambda: R.AdamW([p.double()]),

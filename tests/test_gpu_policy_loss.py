@@ -321,6 +321,25 @@ def test_gradient_over_the_logits(vocab, rows, kind):
         assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("vocab", [18, 5000, 90000])
+def test_rows_far_apart(vocab):
+    """Offsets that pass 32 bits: rows of a buffer of more than 2^32 elements, gradient over the logits.  Which thread holds a column, and
+    with it the order of a row's sums, follows from where the row begins within 16 bytes: the same bits are those of near rows that begin
+    alike."""
+    s = _inputs(3, vocab, "bf16", 21, legal=True)
+    room = torch.empty((1 << 32) + (1 << 17), dtype=torch.bfloat16, device="cuda")
+    far = room.as_strided((3, vocab), (1 << 31, 1), 5)
+    far.copy_(s["logits"])
+    ld = (vocab + 7) // 8 * 8
+    near = torch.empty(3 * ld + 8, dtype=torch.bfloat16, device="cuda").as_strided((3, vocab), (ld, 1), 5)
+    near.copy_(s["logits"])
+    want = _call(dict(s, logits=near))
+    got = _call(dict(s, logits=far), out=far)
+    for p, q in zip(got, want):
+        assert torch.equal(p, q)
+    _check(s, got, _reference(s))
+
+
 def test_no_rows():
     s = {k: v if v is None else v[:0] for k, v in _inputs(3, 8, "fp32", 12).items()}
     got = _call(s)
